@@ -357,6 +357,132 @@ RMI_API int rmi_cov(int dtype,
                     size_t workspace_bytes,
                     void* stream);
 
+/* ---- rows of logits -----------------------------------------------------
+ * The calls below read a row-major matrix of logits, [n_rows][n_cols] of F16, BF16 or F32, whose
+ * rows start `ld` elements apart (ld >= n_cols; what lies between a row's end and the next row is
+ * never read or written).  n_cols is below 2^31 - 65536 and n_rows below 2^31; an element's offset
+ * may pass 32 bits.  Rows of other element types are refused with RMI_ERR_UNSUPPORTED, a
+ * temperature outside [1e-6, 1e6] likewise.  Workspaces follow the rules of rmi_reduce: their
+ * contents need no initialisation, their first RMI_WORKSPACE_TICKET_BYTES bytes are left alone,
+ * and calls that share one are ordered on one stream.  Results are the same bits every time.
+ * None of them has a counterpart in the reference. */
+
+/* The k elements of every row that rank first, in rank order: larger values first, NaN behind
+ * everything, equal values (and -0 and +0) by ascending index, the rule of RMI_RED_ARGMAX.
+ * values[i][j] (dtype) and indices[i][j], both [n_rows][k], get the j-th of row i.  `lse`, if not
+ * NULL, gets the row's log(sum_v exp(x_v / temperature)), which turns the values into probabilities
+ * of the whole row; it is NaN for a row that holds NaN, -inf for one of -inf only, and +inf for one that
+ * holds +inf.  1 <= k <= n_cols and k <= RMI_TOP_K_MAX, or RMI_ERR_BAD_SHAPE. */
+#define RMI_TOP_K_MAX 1024
+RMI_API size_t rmi_top_k_workspace_bytes(int dtype, int64_t n_rows, int64_t n_cols, int k);
+RMI_API int rmi_top_k(int dtype,
+                      int64_t n_rows,
+                      int64_t n_cols,
+                      int64_t ld,
+                      int k,
+                      double temperature,
+                      const void* in,
+                      void* values,
+                      int32_t* indices,
+                      float* lse,
+                      void* workspace,
+                      size_t workspace_bytes,
+                      void* stream);
+
+/* Distillation: the loss of student logits z against the best logits that a teacher left for every
+ * row, t_values[n_rows][k] (of t_dtype: F16, BF16 or F32) at t_indices[n_rows][k]; an index outside
+ * [0, n_cols) marks an entry that is not used.  With T = temperature,
+ *   p_ij  = exp(t_ij / T - L_i),  L_i = log of the sum of exp(t_ij / T) over the used entries, or
+ *           t_lse[i] if t_lse is not NULL (the probabilities then keep the mass that they have over
+ *           the teacher's whole vocabulary: rmi_top_k's lse at the same temperature),
+ *   q_iv  = exp(z_iv / T) / sum_v' exp(z_iv' / T),
+ *   loss[i] = scale * sum_j p_ij (log p_ij - log q_i,t_indices[i][j])       (terms with p = 0 are 0),
+ *   dz_iv = row_grad[i] * scale / T * (q_iv sum_j p_ij - sum of p_ij over j with t_indices[i][j] = v).
+ * scale = T^2 gives the usual weight, T^2 / n_rows the mean over the rows.  row_grad is the gradient
+ * that arrives at loss[i]; NULL stands for ones.  A row without a used entry has loss 0 and gradient
+ * 0, whatever its logits.  A listed token whose logit is -inf makes the loss +inf.  A NaN or a +inf
+ * among the logits makes the row's loss and gradient NaN.  The same token may be listed more than once.
+ *
+ * rmi_distill_loss writes `loss`, and what the caller asks for of the rest: `stats`[n_rows][2] (the
+ * row's maximum and log(sum_v exp((z_v - max) / T)), what rmi_distill_grad wants) and `grad`
+ * ([n_rows][n_cols] of dtype, rows ld_grad apart), which then costs one pass over the logits instead
+ * of two.  rmi_distill_grad writes `grad` from the stats of an earlier rmi_distill_loss with the same
+ * logits, teacher and temperature.  `grad` may be the logits' own memory if ld_grad = ld.
+ * 0 <= k <= RMI_DISTILL_MAX. */
+#define RMI_DISTILL_MAX 1024
+RMI_API size_t rmi_distill_workspace_bytes(int dtype, int64_t n_rows, int64_t n_cols, int k);
+RMI_API int rmi_distill_loss(int dtype,
+                             int t_dtype,
+                             int64_t n_rows,
+                             int64_t n_cols,
+                             int64_t ld,
+                             int k,
+                             double temperature,
+                             double scale,
+                             const void* logits,
+                             const void* t_values,
+                             const int32_t* t_indices,
+                             const float* t_lse,
+                             float* loss,
+                             float* stats,
+                             const float* row_grad,
+                             void* grad,
+                             int64_t ld_grad,
+                             void* workspace,
+                             size_t workspace_bytes,
+                             void* stream);
+RMI_API int rmi_distill_grad(int dtype,
+                             int t_dtype,
+                             int64_t n_rows,
+                             int64_t n_cols,
+                             int64_t ld,
+                             int k,
+                             double temperature,
+                             double scale,
+                             const void* logits,
+                             const void* t_values,
+                             const int32_t* t_indices,
+                             const float* t_lse,
+                             const float* stats,
+                             const float* row_grad,
+                             void* grad,
+                             int64_t ld_grad,
+                             void* stream);
+
+/* One token of every row, drawn with the caller's random number u[i] in [0, 1).  Every row has
+ * settings of its own (arrays of n_rows; a NULL array stands for the value that changes nothing):
+ *   allowed      bit mask of the tokens that may be chosen: bit v % 32 of word v / 32, rows
+ *                ld_allowed words apart; NULL: all.  Tokens of logit -inf or NaN are never chosen.
+ *   temperature  T; a T that is not above 0 takes the token that ranks first (logprob 0), as arg-max
+ *   top_k        then the top_k tokens that rank first (rank order as in rmi_top_k); <= 0: all
+ *   top_p        of those the shortest prefix, in rank order, that has top_p of their mass, and at
+ *                least one: a token stays if the mass that ranks before it is below top_p of theirs
+ *   min_p        of those the ones with at least min_p times the probability of the first
+ * The token is the first in index order at which the cumulative mass of what is left exceeds u times
+ * its sum; a u below 0 or NaN counts as 0, one of 1 or more takes the last token left.  `logprob`, if not
+ * NULL, gets the log of the token's share of what is left.  A row with nothing to choose from (also
+ * n_cols = 0) gets token -1 and logprob -inf.  The weights exp((x - max) / T) are held as whole
+ * multiples of 2^-(62 - ceil(log2(n_cols))), at most 2^-50, of the largest one, so that all sums of them are
+ * exact; tokens of less weight than half of that are never chosen. */
+RMI_API size_t rmi_sample_workspace_bytes(int dtype, int64_t n_rows, int64_t n_cols);
+RMI_API int rmi_sample(int dtype,
+                       int64_t n_rows,
+                       int64_t n_cols,
+                       int64_t ld,
+                       const void* logits,
+                       const uint32_t* allowed,
+                       int64_t ld_allowed,
+                       const float* temperature,
+                       const int32_t* top_k,
+                       const float* top_p,
+                       const float* min_p,
+                       const float* u,
+                       int32_t* token,
+                       float* logprob,
+                       void* workspace,
+                       size_t workspace_bytes,
+                       void* stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

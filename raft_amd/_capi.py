@@ -19,6 +19,8 @@ NOALLOC_SCRATCH_BYTES = 4 << 20
 FLAG_WORKSPACE_ZEROED = 1
 COV_CENTER_DATA = 1
 WORKSPACE_TICKET_BYTES = 65536
+TOP_K_MAX = 1024
+DISTILL_MAX = 1024
 
 # rmi_dtype
 I8, U8, I32, I64, F16, BF16, F32, F64, KVP_I32_F32, KVP_I32_F64, KVP_I64_F32, KVP_I64_F64 = range(12)
@@ -93,6 +95,20 @@ SYMBOLS = {
     "rmi_cov_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int64, C.c_int64]),
     "rmi_cov": (C.c_int, [C.c_int, C.c_int, C.c_int64, C.c_int64, C.c_int, C.c_int, C.c_void_p,
                           C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "rmi_top_k_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int64, C.c_int64, C.c_int]),
+    "rmi_top_k": (C.c_int, [C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_int, C.c_double,
+                            C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t,
+                            C.c_void_p]),
+    "rmi_distill_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int64, C.c_int64, C.c_int]),
+    "rmi_distill_loss": (C.c_int, [C.c_int, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_int,
+                                   C.c_double, C.c_double] + [C.c_void_p] * 8 +
+                         [C.c_int64, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "rmi_distill_grad": (C.c_int, [C.c_int, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_int,
+                                   C.c_double, C.c_double] + [C.c_void_p] * 7 +
+                         [C.c_int64, C.c_void_p]),
+    "rmi_sample_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int64, C.c_int64]),
+    "rmi_sample": (C.c_int, [C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p,
+                             C.c_int64] + [C.c_void_p] * 8 + [C.c_size_t, C.c_void_p]),
 }
 
 _lib = None
