@@ -258,5 +258,294 @@ __device__ Cut find_cut(const T* row, int n, u32 max_key, u64 target, F weigh, u
   }
 }
 
+// ---- candidates: the elements that may be among the first k -------------------------------------
+
+// Where the aligned 16-byte vectors of a row lie: `head` elements come before them, `nv` vectors
+// follow, and what is left after them is shorter than a vector.  Reads of aligned vectors run at
+// the full rate whatever the row's length and stride are.
+template <class T>
+struct Vectors {
+  int head, nv;
+  __device__ __forceinline__ Vectors(const T* row, int n)
+  {
+    const int off = (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / (int)sizeof(T);
+    head          = off < n ? off : n;
+    nv            = (n - head) / In<T>::VEC;
+  }
+  // The index of this thread's element outside the vectors, or -1 (there are at most 2 VEC - 2).
+  __device__ __forceinline__ int extra(int n) const
+  {
+    const int t = (int)threadIdx.x;
+    const int i = t < head ? t : t + nv * In<T>::VEC;
+    return i < n && t < 2 * In<T>::VEC ? i : -1;
+  }
+};
+
+// The bits of 8 (or 4) tokens from `i` on.
+__device__ __forceinline__ u32 mask_bits(const u32* allowed, int i, int words)
+{
+  const int w  = i >> 5;
+  const u32 lo = allowed[w];
+  const u32 hi = allowed[w + 1 < words ? w + 1 : w];
+  return __builtin_amdgcn_alignbit(hi, lo, (u32)i & 31u);
+}
+
+// The largest t, in the upper 16 bits of a key, such that at least `need` of the wave's 64 G keys are
+// t or more; 0 if there are fewer.  Sixteen steps of G comparisons each, counted over the lanes by
+// scalar instructions: no trip to LDS.
+template <int G>
+__device__ __forceinline__ u32 wave_rank(const u32 (&key)[G], int need)
+{
+  u32 t = 0;
+#pragma unroll 1
+  for (u32 bit = 0x80000000u; bit >= 0x10000u; bit >>= 1) {
+    const u32 trial = t | bit;
+    int have        = 0;
+#pragma unroll
+    for (int g = 0; g < G; ++g) have += __popcll(__ballot(key[g] >= trial));
+    if (have >= need) t = trial;
+  }
+  return t;
+}
+
+template <int W, int CAP>
+struct CandidateBox {
+  u64 entries[CAP];
+  u32 bins[kBins];
+  u32 word[W];
+  float max[W];
+  int count;
+  u32 edge;
+};
+
+// How the elements of a row are looked at: kEvery for top_k (NaN and -inf have a rank too), kReal
+// where only what is above -inf counts, kMasked where a bit mask says more.
+enum class Look { kEvery, kReal, kMasked };
+
+// 32-bit ordered key of an fp32 value: the one that candidates are compared by, whatever the type.
+__device__ __forceinline__ u32 key32(float x) { return key_of<float>(x); }
+
+// Keeps of the candidates those that may still be among the first k: their keys are counted in 256
+// equal parts of the range between the least and the largest of them, and everything below the part
+// that holds the k-th is dropped.  Returns the lower edge of that part; box.count is the new count.
+template <int THREADS, int W, int CAP>
+__device__ u32 thin_out(CandidateBox<W, CAP>& box, int count, int k, u32 lo, u32 hi)
+{
+  constexpr int EACH = (CAP + THREADS - 1) / THREADS;
+  const u32 width    = hi - lo;
+  const int bits     = width == 0 ? 0 : 32 - __builtin_clz(width);
+  const int shift    = bits > 8 ? bits - 8 : 0;
+  u64 own[EACH];
+  for (int b = threadIdx.x; b < kBins; b += THREADS) box.bins[b] = 0;
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const int i = e * THREADS + (int)threadIdx.x;
+    own[e]      = i < count ? box.entries[i] : 0;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < EACH; ++e)
+    if (e * THREADS + (int)threadIdx.x < count) atomicAdd(&box.bins[(entry_key(own[e]) - lo) >> shift], 1u);
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    const int l = 63 - (int)threadIdx.x;
+    u32 bin[4], sum = 0;
+#pragma unroll
+    for (int j = 3; j >= 0; --j) sum += bin[j] = box.bins[4 * l + j];
+    u32 upto = sum;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const u32 o = (u32)__shfl_up((int)upto, d, 64);
+      if ((int)threadIdx.x >= d) upto += o;
+    }
+    u32 before = upto - sum;
+    if (before < (u32)k && upto >= (u32)k) {  // one lane: count >= k
+      int b = 3;
+#pragma unroll
+      for (int j = 3; j > 0; --j) {
+        if (b == j && before + bin[j] < (u32)k) {
+          before += bin[j];
+          b = j - 1;
+        }
+      }
+      box.edge  = lo + ((u32)(4 * l + b) << shift);
+      box.count = 0;
+    }
+  }
+  __syncthreads();
+  const u32 edge = box.edge;
+#pragma unroll
+  for (int e = 0; e < EACH; ++e)
+    if (e * THREADS + (int)threadIdx.x < count && entry_key(own[e]) >= edge)
+      box.entries[atomicAdd(&box.count, 1)] = own[e];
+  __syncthreads();
+  return edge;
+}
+
+// A running maximum and sum of exp2((x - m) c) of the elements that one thread sees.
+struct Running {
+  float m = -kInf;
+  float s = 0;
+  __device__ __forceinline__ static float ref(float m) { return fabsf(m) < kInf ? m : 0.0f; }
+  __device__ __forceinline__ void raise(float to, float c)
+  {
+    if (to > m) {
+      s *= __builtin_amdgcn_exp2f((m - ref(to)) * c);
+      m = to;
+    }
+  }
+};
+
+struct Found {
+  int count;   // candidates in the box; more than CAP: they did not fit and the box is of no use
+  u32 tau;     // every element with a key32 of tau or more is in the box; 0: every element
+  float max;   // of the elements that count
+};
+
+// One pass over a row that leaves in `box` at least its first k elements (k <= CAP / 2, or all there
+// are), unordered, with keys of 32 bits.  The first batch of loads sets a threshold: every wave
+// takes the (k / W)-th largest maximum of its vectors, and the least of those is passed by k elements
+// or more.  From then on a vector costs its maximum and a comparison, and few pass; the box is thinned
+// out, and the threshold raised, when it is half full.  `run`, if wanted, is the thread's sum of
+// exponentials for the log-sum-exp, from the same loads.
+template <class T, int THREADS, int CAP, Look LOOK, bool SUM>
+__device__ Found stream_candidates(const T* row, int n, int k, const u32* allowed, float c,
+                                   CandidateBox<THREADS / 64, CAP>& box, Running& run)
+{
+  constexpr int W   = THREADS / 64;
+  constexpr int VEC = In<T>::VEC;
+  constexpr int NV  = 4;
+  const int words   = (n + 31) >> 5;
+  const Vectors<T> vs(row, n);
+  const T* body   = row + vs.head;
+  const int step  = THREADS * NV;
+  const int last  = vs.nv > 0 ? vs.nv - 1 : 0;
+  const bool some = vs.nv > 0;
+  const int wave  = (int)threadIdx.x >> 6;
+
+  float ext       = -kInf;
+  const int ext_i = vs.extra(n);
+  bool ext_on     = ext_i >= 0;
+  if (ext_on) {
+    ext = widen(row + ext_i);
+    if (LOOK == Look::kMasked && ((allowed[ext_i >> 5] >> (ext_i & 31)) & 1u) == 0) ext_on = false;
+    if (LOOK != Look::kEvery && !(ext > -kInf)) ext_on = false;
+  }
+  if (!ext_on) ext = -kInf;
+  if (SUM && ext_on) {
+    run.raise(ext, c);
+    run.s += __builtin_amdgcn_exp2f((ext - Running::ref(run.m)) * c);
+  }
+  float seen_max = fmaxf(ext, -kInf);
+
+  u32x4 now[NV], next[NV];
+  auto fetch = [&](u32x4(&w)[NV], int first) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      int v = first + i * THREADS + (int)threadIdx.x;
+      v     = v < last ? v : last;
+      w[i]  = load16(body + (int64_t)v * VEC);
+    }
+  };
+  auto unpack = [&](const u32x4& w, int v, float(&x)[VEC]) {
+    static_for<VEC>([&](auto j) { x[j] = (float)In<T>::template get<j>(w); });
+    if constexpr (LOOK == Look::kMasked) {
+      const u32 bits = mask_bits(allowed, vs.head + v * VEC, words);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) x[j] = (bits >> j) & 1u ? x[j] : -kInf;
+    }
+  };
+  auto most = [&](const float(&x)[VEC]) {
+    float m = x[0];
+#pragma unroll
+    for (int j = 1; j < VEC; ++j) m = fmaxf(m, x[j]);
+    return fmaxf(m, -kInf);  // NaN throughout: -inf
+  };
+  auto put = [&](float x, int i) {
+    const int at = atomicAdd(&box.count, 1);
+    if (at < CAP) box.entries[at] = entry_of(key32(x), (u32)i);
+  };
+
+  if (threadIdx.x == 0) box.count = 0;
+  if (some) fetch(now, 0);
+  u32 tau;
+  {
+    u32 key[NV + 1];
+    key[NV] = ext_on && ext > -kInf ? key32(ext) : 0u;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int v = i * THREADS + (int)threadIdx.x;
+      key[i]      = 0;
+      if (v < vs.nv) {
+        float x[VEC];
+        unpack(now[i], v, x);
+        const float m = most(x);
+        key[i]        = m > -kInf ? key32(m) : 0u;
+      }
+    }
+    tau = wave_rank<NV + 1>(key, (k + W - 1) / W);
+    if ((threadIdx.x & 63) == 0) box.word[wave] = tau;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < W; ++w) tau = tau < box.word[w] ? tau : box.word[w];
+  }
+  float at_least = tau != 0 ? as_f32((tau >> 31) ? tau & 0x7fffffffu : ~tau) : -kInf;
+  if (ext_on && (tau == 0 || ext >= at_least)) put(ext, ext_i);
+
+  for (int first = 0; first < vs.nv; first += step) {
+    fetch(next, first + step);  // unconditional: a load under a branch would be waited for at its end
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int v = first + i * THREADS + (int)threadIdx.x;
+      if (v < vs.nv) {
+        float x[VEC];
+        unpack(now[i], v, x);
+        const float m = most(x);
+        seen_max      = fmaxf(seen_max, m);
+        if constexpr (SUM) {
+          run.raise(m, c);
+          const float ref = Running::ref(run.m);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) run.s += __builtin_amdgcn_exp2f((x[j] - ref) * c);
+        }
+        if (tau == 0 || m >= at_least) {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            const bool on = LOOK == Look::kEvery ? (tau == 0 || x[j] >= at_least)
+                                                 : (x[j] > -kInf && x[j] >= at_least);
+            if (on) put(x[j], vs.head + v * VEC + j);
+          }
+        }
+      }
+    }
+    if (first + step < vs.nv) {
+      __syncthreads();
+      const int count = box.count;
+      if (count > CAP) {  // they do not fit: what is left of the row is read for its maximum and sum
+        tau      = ~0u;
+        at_least = kInf;
+      } else if (count > CAP / 2 && count >= k) {
+        u32 top = 0, low = ~0u;
+        for (int i = threadIdx.x; i < count; i += THREADS) {
+          const u32 e = entry_key(box.entries[i]);
+          top         = top > e ? top : e;
+          low         = low < e ? low : e;
+        }
+        top = block_all<W>(top, MaxF{}, box.word);
+        low = ~block_all<W>(~low, MaxF{}, box.word);
+        tau = thin_out<THREADS>(box, count, k, low, top);
+        if (tau < 0x00800000u) tau = 0;  // at or below the key of -inf: NaN's and -inf's own ranks
+        if (tau != 0) at_least = as_f32((tau >> 31) ? tau & 0x7fffffffu : ~tau);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < NV; ++i) now[i] = next[i];
+    }
+  }
+  const float m = block_all<W>(seen_max, MaxF{}, box.max);
+  __syncthreads();
+  return Found{box.count, tau, m};
+}
+
 }  // namespace logits
 }  // namespace rmi

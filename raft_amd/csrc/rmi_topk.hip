@@ -37,43 +37,17 @@ __device__ __forceinline__ void sort_entries(u64* e, int size)
   __syncthreads();
 }
 
-// One workgroup per row.  The row is swept for its maximum, for the sum of its exponentials, for
-// the key of its k-th element (8 bits of the key a sweep) and for the elements themselves.
-template <class T, int THREADS>
-__global__ __launch_bounds__(THREADS) void top_k_kernel(TopKArgs a)
+// What a row's candidates do not fit: the key of the k-th element by sweeps of the row, 8 bits of
+// the key a sweep, then the elements above it and the first ones that have it, in index order.
+template <class T, int THREADS, int CAP>
+__device__ __noinline__ void gather_exact(const T* row, int n, int k, float max, CandidateBox<THREADS / 64, CAP>& box)
 {
   constexpr int W   = THREADS / 64;
   constexpr int VEC = In<T>::VEC;
-  __shared__ u64 bins[kBins + 2];
-  __shared__ u64 entries[RMI_TOP_K_MAX];
-  __shared__ u64 box[W];
-  __shared__ int filled;
-  const int r   = blockIdx.x;
-  const T* row  = static_cast<const T*>(a.in) + (int64_t)r * a.ld;
-  const int n   = a.n_cols;
-  float m       = -kInf;
-  u32 top       = 0;
-  sweep<T, THREADS>(row, n, [&](float x, int) {
-    m           = fmaxf(m, x);
-    const u32 k = key_of<T>(x);
-    top         = top > k ? top : k;
-  });
-  m   = block_all<W>(m, MaxF{}, reinterpret_cast<float*>(box));
-  top = block_all<W>(top, MaxF{}, reinterpret_cast<u32*>(box));
-  if (a.lse != nullptr) {
-    const float ref = fabsf(m) < kInf ? m : 0.0f;
-    float s         = 0;
-    sweep<T, THREADS>(row, n, [&](float x, int) { s += __builtin_amdgcn_exp2f((x - ref) * a.scale); });
-    const double all = block_all<W>((double)s, AddF{}, reinterpret_cast<double*>(box));
-    if (threadIdx.x == 0)
-      a.lse[r] = all == all && fabsf(m) == kInf ? m : (float)((double)ref * a.inv_t + log(all));
-  }
-  const Cut cut = find_cut<T, THREADS>(row, n, top, (u64)a.k, [](float, int) { return (u64)1; }, bins);
-  const int want = a.k - (int)cut.above;  // elements with the cut's own key, from the lowest index on
-  int size = 1;
-  while (size < a.k) size <<= 1;
-  if (threadIdx.x == 0) filled = 0;
-  for (int i = threadIdx.x; i < size; i += THREADS) entries[i] = 0;
+  const Cut cut     = find_cut<T, THREADS>(row, n, key_of<T>(max), (u64)k, [](float, int) { return (u64)1; }, box.entries);
+  const int want    = k - (int)cut.above;  // elements with the cut's own key, from the lowest index on
+  __syncthreads();
+  if (threadIdx.x == 0) box.count = 0;
   __syncthreads();
   int seen = 0;
   ordered_sweep<T, THREADS>(row, n, [&](int at, const float(&x)[VEC], int count) {
@@ -81,37 +55,87 @@ __global__ __launch_bounds__(THREADS) void top_k_kernel(TopKArgs a)
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
       if (j >= count) continue;
-      const u32 k = key_of<T>(x[j]);
-      ties += k == cut.key;
-      if (k > cut.key) entries[atomicAdd(&filled, 1)] = entry_of(k, (u32)(at + j));
+      const u32 key = key_of<T>(x[j]);
+      ties += key == cut.key;
+      if (key > cut.key) box.entries[atomicAdd(&box.count, 1)] = entry_of(key32(x[j]), (u32)(at + j));
     }
     if (seen < want) {
       int all;
-      int rank = seen + block_before<W>(ties, reinterpret_cast<int*>(box), all);
+      int rank = seen + block_before<W>(ties, reinterpret_cast<int*>(box.word), all);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         if (j >= count || key_of<T>(x[j]) != cut.key) continue;
-        if (rank < want) entries[atomicAdd(&filled, 1)] = entry_of(cut.key, (u32)(at + j));
+        if (rank < want) box.entries[atomicAdd(&box.count, 1)] = entry_of(key32(x[j]), (u32)(at + j));
         ++rank;
       }
       seen += all;
     }
     return true;
   });
-  sort_entries<THREADS>(entries, size);
+  __syncthreads();
+}
+
+// One workgroup per row: one pass over the row for its candidates and its sum of exponentials; the
+// candidates are thinned out to little more than k and sorted in LDS.
+template <class T, int THREADS, bool SUM>
+__global__ __launch_bounds__(THREADS) void top_k_kernel(TopKArgs a)
+{
+  constexpr int W   = THREADS / 64;
+  constexpr int CAP = 8 * THREADS;
+  __shared__ CandidateBox<W, CAP> box;
+  __shared__ double sums[W];
+  const int r  = blockIdx.x;
+  const T* row = static_cast<const T*>(a.in) + (int64_t)r * a.ld;
+  const int n  = a.n_cols;
+  Running run;
+  const Found f = stream_candidates<T, THREADS, CAP, Look::kEvery, SUM>(row, n, a.k, nullptr, a.scale, box, run);
+  if constexpr (SUM) {
+    const float ref  = Running::ref(f.max);
+    const float own  = run.s * __builtin_amdgcn_exp2f((run.m - ref) * a.scale);
+    const double all = block_all<W>(run.m > -kInf ? (double)own : (double)run.s, AddF{}, sums);
+    if (threadIdx.x == 0)
+      a.lse[r] = all == all && fabsf(f.max) == kInf ? f.max : (float)((double)ref * a.inv_t + log(all));
+  }
+  int count = f.count;
+  if (count > CAP) {
+    gather_exact<T, THREADS, CAP>(row, n, a.k, f.max, box);
+    count = a.k;
+  } else if (count > a.k) {
+    thin_out<THREADS>(box, count, a.k, f.tau, key32(f.max));
+    count = box.count;
+  }
+  int size = 1;
+  while (size < count) size <<= 1;
+  for (int i = count + (int)threadIdx.x; i < size; i += THREADS) box.entries[i] = 0;
+  sort_entries<THREADS>(box.entries, size);
   for (int j = threadIdx.x; j < a.k; j += THREADS) {
-    const u32 i       = entry_index(entries[j]);
+    const u32 i       = entry_index(box.entries[j]);
     const int64_t out = (int64_t)r * a.k + j;
     static_cast<T*>(a.values)[out] = row[i];
     a.indices[out]                 = (int32_t)i;
   }
 }
 
+template <class T, int THREADS>
+int launch_rows(const TopKArgs& a, hipStream_t st)
+{
+  const dim3 grid((unsigned)a.n_rows), block(THREADS);
+  if (a.lse != nullptr)
+    hipLaunchKernelGGL((top_k_kernel<T, THREADS, true>), grid, block, 0, st, a);
+  else
+    hipLaunchKernelGGL((top_k_kernel<T, THREADS, false>), grid, block, 0, st, a);
+  return hipGetLastError() == hipSuccess ? RMI_OK : RMI_ERR_LAUNCH;
+}
+
 template <class T>
 int launch(const TopKArgs& a, hipStream_t st)
 {
-  hipLaunchKernelGGL((top_k_kernel<T, 256>), dim3((unsigned)a.n_rows), dim3(256), 0, st, a);
-  return hipGetLastError() == hipSuccess ? RMI_OK : RMI_ERR_LAUNCH;
+  // A workgroup of 256 threads sets its threshold from 1024 vectors' maxima, which is sharp while k is
+  // a quarter of that; few long rows want all the loads that one CU can have in flight.
+  const bool few = a.n_rows <= 512 && (int64_t)a.n_cols * (int)sizeof(T) >= 32768;
+  if (a.k > 512 || few) return launch_rows<T, 1024>(a, st);
+  if (a.k > 256) return launch_rows<T, 512>(a, st);
+  return launch_rows<T, 256>(a, st);
 }
 
 }  // namespace
