@@ -308,12 +308,19 @@ __device__ __forceinline__ u32 wave_rank(const u32 (&key)[G], int need)
   return t;
 }
 
-template <int W, int CAP>
+// What a workgroup of W waves keeps in LDS while it looks for candidates: whole vectors that hold
+// one (`hits`), and the candidates themselves.
+template <int W>
 struct CandidateBox {
-  u64 entries[CAP];
+  static constexpr int kHits    = 128 * W;
+  static constexpr int kEntries = 256 * W;
+  u64 entries[kEntries];
+  u32x4 hit[kHits];
+  int hit_at[kHits];  // the index of a vector's first element
   u32 bins[kBins];
   u32 word[W];
   float max[W];
+  int hits;
   int count;
   u32 edge;
 };
@@ -328,10 +335,11 @@ __device__ __forceinline__ u32 key32(float x) { return key_of<float>(x); }
 // Keeps of the candidates those that may still be among the first k: their keys are counted in 256
 // equal parts of the range between the least and the largest of them, and everything below the part
 // that holds the k-th is dropped.  Returns the lower edge of that part; box.count is the new count.
-template <int THREADS, int W, int CAP>
-__device__ u32 thin_out(CandidateBox<W, CAP>& box, int count, int k, u32 lo, u32 hi)
+template <int W>
+__device__ u32 thin_out(CandidateBox<W>& box, int count, int k, u32 lo, u32 hi)
 {
-  constexpr int EACH = (CAP + THREADS - 1) / THREADS;
+  constexpr int THREADS = 64 * W;
+  constexpr int EACH    = CandidateBox<W>::kEntries / THREADS;
   const u32 width    = hi - lo;
   const int bits     = width == 0 ? 0 : 32 - __builtin_clz(width);
   const int shift    = bits > 8 ? bits - 8 : 0;
@@ -382,46 +390,111 @@ __device__ u32 thin_out(CandidateBox<W, CAP>& box, int count, int k, u32 lo, u32
   return edge;
 }
 
-// A running maximum and sum of exp2((x - m) c) of the elements that one thread sees.
+// From here on the wave's maxima ignore signalling NaNs as they ignore quiet ones (bit 9 of the MODE
+// register, IEEE, off).  With it on, fmaxf needs an instruction per element that makes them quiet
+// first.  Called once, at the start of a kernel.
+__device__ __forceinline__ void maxima_ignore_nan() { __builtin_amdgcn_s_setreg(1 | (9 << 6), 0); }
+
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+// The largest of a vector's elements, NaN ignored (NaN if there is nothing else).
+template <int N>
+__device__ __forceinline__ float max_of(const float (&x)[N])
+{
+  static_assert(N == 4 || N == 8, "vectors of 4 or 8 elements");
+  if constexpr (N == 8)
+    return max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), max3(x[6], x[7], x[7]));
+  else
+    return max3(max3(x[0], x[1], x[2]), x[3], x[3]);
+}
+
+// A running maximum and sum of exp2((x - m) c) of the elements that one thread sees.  The terms are
+// exp2(fma(x, c, -r)) with r = fl(m c): one rounding each, and r's own drops out of the sum's
+// logarithm, which is taken against r.  Maxima so large that m c overflows (rows of the type's lowest
+// value) take the difference first.
 struct Running {
+  static constexpr float kLarge = 1e30f;
   float m = -kInf;
+  float r = 0;
   float s = 0;
   __device__ __forceinline__ static float ref(float m) { return fabsf(m) < kInf ? m : 0.0f; }
   __device__ __forceinline__ void raise(float to, float c)
   {
     if (to > m) {
-      s *= __builtin_amdgcn_exp2f((m - ref(to)) * c);
+      const float q = ref(to) * c;
+      s *= fabsf(to) < kLarge && fabsf(m) < kLarge ? __builtin_amdgcn_exp2f(r - q)
+                                                   : __builtin_amdgcn_exp2f((m - ref(to)) * c);
       m = to;
+      r = q;
     }
+  }
+  // After raise() with at least the largest of them.
+  template <int N, int V>
+  __device__ __forceinline__ void add(const float (&x)[N][V], float c)
+  {
+    float t[2] = {0, 0};
+    if (__builtin_expect(fabsf(m) < kLarge, 1)) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) t[j & 1] += __builtin_amdgcn_exp2f(fmaf(x[i][j], c, -r));
+    } else {
+      const float at = ref(m);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) t[j & 1] += __builtin_amdgcn_exp2f((x[i][j] - at) * c);
+    }
+    s += t[0] + t[1];
+  }
+  // This thread's sum against the maximum `top` of all; top's own r is ref(top) * c.
+  __device__ __forceinline__ double against(float top, float c) const
+  {
+    const float q = ref(top) * c;
+    if (!(m > -kInf)) return (double)s;  // nothing, or NaN alone
+    return (double)(fabsf(top) < kLarge && fabsf(m) < kLarge ? s * __builtin_amdgcn_exp2f(r - q)
+                                                             : s * __builtin_amdgcn_exp2f((m - ref(top)) * c));
+  }
+  // log of sum exp(x / T) from all = the sum over the threads of against(top)
+  __device__ __forceinline__ static double log_sum(float top, float c, double inv_t, double all)
+  {
+    if (all == all && fabsf(top) == kInf) return (double)top;
+    return (fabsf(top) < kLarge ? (double)(ref(top) * c) * kLn2 : (double)ref(top) * inv_t) + log(all);
   }
 };
 
 struct Found {
-  int count;   // candidates in the box; more than CAP: they did not fit and the box is of no use
+  bool all;    // the box holds the candidates; otherwise they did not fit and it is of no use
+  int count;   // how many
   u32 tau;     // every element with a key32 of tau or more is in the box; 0: every element
   float max;   // of the elements that count
 };
 
-// One pass over a row that leaves in `box` at least its first k elements (k <= CAP / 2, or all there
-// are), unordered, with keys of 32 bits.  The first batch of loads sets a threshold: every wave
-// takes the (k / W)-th largest maximum of its vectors, and the least of those is passed by k elements
-// or more.  From then on a vector costs its maximum and a comparison, and few pass; the box is thinned
-// out, and the threshold raised, when it is half full.  `run`, if wanted, is the thread's sum of
+// One pass over a row that leaves in `box` at least its first k elements (k <= 64 W, or all there
+// are), unordered, with keys of 32 bits.  The first NV loads of every thread set a threshold: every
+// wave takes the (k / W)-th largest of its 256 maxima over NV / 4 vectors, and the least of the waves' is
+// passed by k elements or more.  From then on a vector costs its maximum and a comparison; the few that
+// pass are put aside whole and looked at element by element between the batches, all lanes at once (an
+// element taken out where it is found costs a whole wave some twenty instructions).  The threshold is
+// raised when twice k elements have gathered.  A vector's registers are loaded again as soon as it has been
+// looked at, so NV loads per thread are in flight throughout.  `run`, if wanted, is the thread's sum of
 // exponentials for the log-sum-exp, from the same loads.
-template <class T, int THREADS, int CAP, Look LOOK, bool SUM>
-__device__ Found stream_candidates(const T* row, int n, int k, const u32* allowed, float c,
-                                   CandidateBox<THREADS / 64, CAP>& box, Running& run)
+template <class T, int W, int NV, Look LOOK, bool SUM>
+__device__ __forceinline__ Found stream_candidates(const T* row, int n, int k, const u32* allowed, float c,
+                                                   CandidateBox<W>& box, Running& run)
 {
-  constexpr int W   = THREADS / 64;
-  constexpr int VEC = In<T>::VEC;
-  constexpr int NV  = 4;
-  const int words   = (n + 31) >> 5;
+  constexpr int THREADS = 64 * W;
+  constexpr int VEC     = In<T>::VEC;
+  constexpr int GROUP   = NV / 4;
+  const int words       = (n + 31) >> 5;
   const Vectors<T> vs(row, n);
   const T* body   = row + vs.head;
-  const int step  = THREADS * NV;
   const int last  = vs.nv > 0 ? vs.nv - 1 : 0;
-  const bool some = vs.nv > 0;
-  const int wave  = (int)threadIdx.x >> 6;
+  const int tid   = (int)threadIdx.x;
 
   float ext       = -kInf;
   const int ext_i = vs.extra(n);
@@ -433,118 +506,183 @@ __device__ Found stream_candidates(const T* row, int n, int k, const u32* allowe
   }
   if (!ext_on) ext = -kInf;
   if (SUM && ext_on) {
+    const float one[1][1] = {{ext}};
     run.raise(ext, c);
-    run.s += __builtin_amdgcn_exp2f((ext - Running::ref(run.m)) * c);
+    run.add(one, c);
   }
-  float seen_max = fmaxf(ext, -kInf);
+  float seen_max = ext > -kInf ? ext : -kInf;
 
-  u32x4 now[NV], next[NV];
-  auto fetch = [&](u32x4(&w)[NV], int first) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      int v = first + i * THREADS + (int)threadIdx.x;
-      v     = v < last ? v : last;
-      w[i]  = load16(body + (int64_t)v * VEC);
-    }
+  // Vectors are addressed by a byte offset from the batch's first one, which is the same for all lanes:
+  // no 64-bit arithmetic per load.  Offsets are held within the row.
+  constexpr int BATCH = THREADS * NV;
+  u32x4 now[NV];
+  auto fetch = [&](int first, int i) {
+    const int left = last - first;
+    const u32 room = (u32)(left < BATCH ? left : BATCH) * 16u;
+    u32 off        = (u32)(i * THREADS + tid) * 16u;
+    off            = off < room ? off : room;
+    return __builtin_nontemporal_load(
+      reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(body + (int64_t)first * VEC) + off));
   };
-  auto unpack = [&](const u32x4& w, int v, float(&x)[VEC]) {
+  // The elements of a vector; what does not count, or lies behind the last vector, is -inf.
+  auto unpack = [&](const u32x4& w, int v, float(&x)[VEC], bool whole) {
     static_for<VEC>([&](auto j) { x[j] = (float)In<T>::template get<j>(w); });
     if constexpr (LOOK == Look::kMasked) {
-      const u32 bits = mask_bits(allowed, vs.head + v * VEC, words);
+      const int at   = v < last ? v : last;
+      const u32 bits = mask_bits(allowed, vs.head + at * VEC, words);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) x[j] = (bits >> j) & 1u ? x[j] : -kInf;
     }
-  };
-  auto most = [&](const float(&x)[VEC]) {
-    float m = x[0];
+    if (!whole && v >= vs.nv) {
 #pragma unroll
-    for (int j = 1; j < VEC; ++j) m = fmaxf(m, x[j]);
-    return fmaxf(m, -kInf);  // NaN throughout: -inf
+      for (int j = 0; j < VEC; ++j) x[j] = -kInf;
+    }
   };
   auto put = [&](float x, int i) {
     const int at = atomicAdd(&box.count, 1);
-    if (at < CAP) box.entries[at] = entry_of(key32(x), (u32)i);
+    if (at < CandidateBox<W>::kEntries) box.entries[at] = entry_of(key32(x), (u32)i);
   };
+  // without a threshold (tau = 0) every element passes, NaN too
+  auto value_at = [](u32 key) { return key != 0 ? as_f32((key >> 31) ? key & 0x7fffffffu : ~key) : -kInf; };
 
-  if (threadIdx.x == 0) box.count = 0;
-  if (some) fetch(now, 0);
-  u32 tau;
-  {
-    u32 key[NV + 1];
-    key[NV] = ext_on && ext > -kInf ? key32(ext) : 0u;
+  if (tid == 0) box.count = box.hits = 0;
+  if (vs.nv > 0) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int v = i * THREADS + (int)threadIdx.x;
-      key[i]      = 0;
-      if (v < vs.nv) {
-        float x[VEC];
-        unpack(now[i], v, x);
-        const float m = most(x);
-        key[i]        = m > -kInf ? key32(m) : 0u;
+    for (int i = 0; i < NV; ++i) now[i] = fetch(0, i);
+  }
+  u32 tau        = 0;
+  float at_least = -kInf;
+  bool fits      = true;
+  float m[NV];
+  // the vectors' maxima, and their share of the sum, two vectors at a time
+  auto take_in = [&](int first, bool whole) {
+    constexpr int PAIR = 2;
+#pragma unroll
+    for (int i = 0; i < NV; i += PAIR) {
+      if (!whole && first + i * THREADS >= vs.nv) {
+        m[i] = m[i + 1] = -kInf;
+        continue;
+      }
+      float x[PAIR][VEC];
+#pragma unroll
+      for (int p = 0; p < PAIR; ++p) {
+        unpack(now[i + p], first + (i + p) * THREADS + tid, x[p], whole);
+        m[i + p] = max_of(x[p]);
+      }
+      const float most = max3(m[i], m[i + 1], -kInf);
+      seen_max         = max3(seen_max, most, most);
+      if constexpr (SUM) {
+        run.raise(most, c);
+        run.add(x, c);
       }
     }
-    tau = wave_rank<NV + 1>(key, (k + W - 1) / W);
-    if ((threadIdx.x & 63) == 0) box.word[wave] = tau;
+  };
+  // puts vectors aside that hold a candidate, and loads the next batch in their place.  The places are
+  // counted over the wave's lanes; one lane takes room for all of them.
+  auto put_aside = [&](int first, bool whole, bool more) {
+    u32 on = 0;
+    int total = 0, place[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int v = first + i * THREADS + tid;
+      // a vector of NaN alone has rank, too, where everything passes
+      const bool hit = (m[i] >= at_least || (LOOK == Look::kEvery && tau == 0 && fits)) && (whole || v < vs.nv);
+      const u64 all  = __ballot(hit);
+      place[i]       = total + (int)__builtin_amdgcn_mbcnt_hi((u32)(all >> 32), __builtin_amdgcn_mbcnt_lo((u32)all, 0u));
+      total += __popcll(all);
+      on |= hit ? 1u << i : 0u;
+    }
+    if (total != 0) {
+      int base = 0;
+      if ((tid & 63) == 0) base = atomicAdd(&box.hits, total);
+      base = __builtin_amdgcn_readfirstlane(base);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int at = base + place[i];
+        if (((on >> i) & 1u) != 0 && at < CandidateBox<W>::kHits) {
+          box.hit[at]    = now[i];
+          box.hit_at[at] = vs.head + (first + i * THREADS + tid) * VEC;
+        }
+      }
+    }
+    if (more) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) now[i] = fetch(first + BATCH, i);
+    }
+  };
+  auto first_threshold = [&]() {
+    u32 key[5];
+    key[4] = ext_on && ext > -kInf ? key32(ext) : 0u;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      float o = -kInf;
+#pragma unroll
+      for (int i = g * GROUP; i < (g + 1) * GROUP; ++i) o = max3(o, m[i], m[i]);
+      key[g] = o > -kInf ? key32(o) : 0u;
+    }
+    tau = wave_rank<5>(key, (k + W - 1) / W);
+    if ((tid & 63) == 0) box.word[tid >> 6] = tau;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < W; ++w) tau = tau < box.word[w] ? tau : box.word[w];
-  }
-  float at_least = tau != 0 ? as_f32((tau >> 31) ? tau & 0x7fffffffu : ~tau) : -kInf;
-  if (ext_on && (tau == 0 || ext >= at_least)) put(ext, ext_i);
-
-  for (int first = 0; first < vs.nv; first += step) {
-    fetch(next, first + step);  // unconditional: a load under a branch would be waited for at its end
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int v = first + i * THREADS + (int)threadIdx.x;
-      if (v < vs.nv) {
-        float x[VEC];
-        unpack(now[i], v, x);
-        const float m = most(x);
-        seen_max      = fmaxf(seen_max, m);
-        if constexpr (SUM) {
-          run.raise(m, c);
-          const float ref = Running::ref(run.m);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) run.s += __builtin_amdgcn_exp2f((x[j] - ref) * c);
-        }
-        if (tau == 0 || m >= at_least) {
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const bool on = LOOK == Look::kEvery ? (tau == 0 || x[j] >= at_least)
-                                                 : (x[j] > -kInf && x[j] >= at_least);
-            if (on) put(x[j], vs.head + v * VEC + j);
-          }
-        }
+    at_least = value_at(tau);
+    if (ext_on && (tau == 0 || ext >= at_least)) put(ext, ext_i);
+  };
+  // between two batches: the vectors put aside are looked at element by element
+  auto gather = [&](bool more) {
+    __syncthreads();
+    const int hits = box.hits;
+    if (hits > CandidateBox<W>::kHits) {  // what is left of the row is read for its maximum and sum
+      fits     = false;
+      at_least = __builtin_nanf("");
+    } else if (hits > (more ? CandidateBox<W>::kHits / 4 : 0)) {
+      const T* flat = reinterpret_cast<const T*>(box.hit);
+      for (int i = tid; i < hits * VEC; i += THREADS) {
+        const float x = (float)In<T>::ld(flat + i);
+        const int at  = box.hit_at[i / VEC] + i % VEC;
+        bool on       = LOOK == Look::kEvery ? (tau == 0 || x >= at_least) : (x > -kInf && x >= at_least);
+        if (LOOK == Look::kMasked && on) on = ((allowed[at >> 5] >> (at & 31)) & 1u) != 0;
+        if (on) put(x, at);
       }
-    }
-    if (first + step < vs.nv) {
       __syncthreads();
       const int count = box.count;
-      if (count > CAP) {  // they do not fit: what is left of the row is read for its maximum and sum
-        tau      = ~0u;
-        at_least = kInf;
-      } else if (count > CAP / 2 && count >= k) {
+      if (tid == 0) box.hits = 0;
+      if (count > CandidateBox<W>::kEntries) {
+        fits     = false;
+        at_least = __builtin_nanf("");
+      } else if (more && count >= 2 * k && count >= THREADS) {
         u32 top = 0, low = ~0u;
-        for (int i = threadIdx.x; i < count; i += THREADS) {
+        for (int i = tid; i < count; i += THREADS) {
           const u32 e = entry_key(box.entries[i]);
           top         = top > e ? top : e;
           low         = low < e ? low : e;
         }
         top = block_all<W>(top, MaxF{}, box.word);
         low = ~block_all<W>(~low, MaxF{}, box.word);
-        tau = thin_out<THREADS>(box, count, k, low, top);
+        tau = thin_out<W>(box, count, k, low, top);
         if (tau < 0x00800000u) tau = 0;  // at or below the key of -inf: NaN's and -inf's own ranks
-        if (tau != 0) at_least = as_f32((tau >> 31) ? tau & 0x7fffffffu : ~tau);
+        at_least = value_at(tau);
       }
       __syncthreads();
-#pragma unroll
-      for (int i = 0; i < NV; ++i) now[i] = next[i];
     }
+  };
+  int first = 0;
+  for (; first + BATCH <= vs.nv; first += BATCH) {
+    take_in(first, true);
+    if (first == 0) first_threshold();
+    const bool more = first + BATCH < vs.nv;
+    put_aside(first, true, more);
+    gather(more);
   }
-  const float m = block_all<W>(seen_max, MaxF{}, box.max);
+  if (first < vs.nv || vs.nv == 0) {
+    take_in(first, false);
+    if (first == 0) first_threshold();
+    put_aside(first, false, false);
+    gather(false);
+  }
+  const float top = block_all<W>(seen_max, MaxF{}, box.max);
   __syncthreads();
-  return Found{box.count, tau, m};
+  return Found{fits, box.count, tau, top};
 }
 
 }  // namespace logits

@@ -1,6 +1,7 @@
 // rmi_top_k / rmi_top_k_workspace_bytes (include/rmi_reduce.h): the k elements of every row that
 // rank first, in rank order, and the row's log-sum-exp.
 #include "rmi_logits.hpp"
+#include "rmi_normalize.hpp"
 
 namespace rmi {
 namespace logits {
@@ -39,11 +40,11 @@ __device__ __forceinline__ void sort_entries(u64* e, int size)
 
 // What a row's candidates do not fit: the key of the k-th element by sweeps of the row, 8 bits of
 // the key a sweep, then the elements above it and the first ones that have it, in index order.
-template <class T, int THREADS, int CAP>
-__device__ __noinline__ void gather_exact(const T* row, int n, int k, float max, CandidateBox<THREADS / 64, CAP>& box)
+template <class T, int W>
+__device__ __noinline__ void gather_exact(const T* row, int n, int k, float max, CandidateBox<W>& box)
 {
-  constexpr int W   = THREADS / 64;
-  constexpr int VEC = In<T>::VEC;
+  constexpr int THREADS = 64 * W;
+  constexpr int VEC     = In<T>::VEC;
   const Cut cut     = find_cut<T, THREADS>(row, n, key_of<T>(max), (u64)k, [](float, int) { return (u64)1; }, box.entries);
   const int want    = k - (int)cut.above;  // elements with the cut's own key, from the lowest index on
   __syncthreads();
@@ -77,65 +78,80 @@ __device__ __noinline__ void gather_exact(const T* row, int n, int k, float max,
 
 // One workgroup per row: one pass over the row for its candidates and its sum of exponentials; the
 // candidates are thinned out to little more than k and sorted in LDS.
-template <class T, int THREADS, bool SUM>
-__global__ __launch_bounds__(THREADS) void top_k_kernel(TopKArgs a)
+template <class T, int W, int NV, bool SUM>
+__global__ __launch_bounds__(64 * W, 4) void top_k_kernel(TopKArgs a)
 {
-  constexpr int W   = THREADS / 64;
-  constexpr int CAP = 8 * THREADS;
-  __shared__ CandidateBox<W, CAP> box;
+  constexpr int THREADS = 64 * W;
+  __shared__ CandidateBox<W> box;
   __shared__ double sums[W];
+  maxima_ignore_nan();
   const int r  = blockIdx.x;
   const T* row = static_cast<const T*>(a.in) + (int64_t)r * a.ld;
   const int n  = a.n_cols;
   Running run;
-  const Found f = stream_candidates<T, THREADS, CAP, Look::kEvery, SUM>(row, n, a.k, nullptr, a.scale, box, run);
+  const Found f = stream_candidates<T, W, NV, Look::kEvery, SUM>(row, n, a.k, nullptr, a.scale, box, run);
   if constexpr (SUM) {
-    const float ref  = Running::ref(f.max);
-    const float own  = run.s * __builtin_amdgcn_exp2f((run.m - ref) * a.scale);
-    const double all = block_all<W>(run.m > -kInf ? (double)own : (double)run.s, AddF{}, sums);
-    if (threadIdx.x == 0)
-      a.lse[r] = all == all && fabsf(f.max) == kInf ? f.max : (float)((double)ref * a.inv_t + log(all));
+    const double all = block_all<W>(run.against(f.max, a.scale), AddF{}, sums);
+    if (threadIdx.x == 0) a.lse[r] = (float)Running::log_sum(f.max, a.scale, a.inv_t, all);
   }
   int count = f.count;
-  if (count > CAP) {
-    gather_exact<T, THREADS, CAP>(row, n, a.k, f.max, box);
+  if (!f.all) {
+    gather_exact<T, W>(row, n, a.k, f.max, box);
     count = a.k;
-  } else if (count > a.k) {
-    thin_out<THREADS>(box, count, a.k, f.tau, key32(f.max));
+  } else if (count > THREADS && count > a.k) {
+    thin_out<W>(box, count, a.k, f.tau, key32(f.max));
     count = box.count;
+  }
+  auto write = [&](int j, u64 e) {
+    const u32 key     = entry_key(e);
+    const u32 i       = entry_index(e);
+    const int64_t out = (int64_t)r * a.k + j;
+    // the key says the value but for the sign of a zero and the bits of a NaN
+    if (key == 0 || key == 0x80000000u)
+      static_cast<T*>(a.values)[out] = row[i];
+    else
+      Put<T>::st(static_cast<T*>(a.values) + out, value_of<float>(key));
+    a.indices[out] = (int32_t)i;
+  };
+  if (count <= THREADS) {
+    // a thread per candidate counts those that rank before it: no barrier, and every lane reads the
+    // same place in LDS
+    const u64 own = (int)threadIdx.x < count ? box.entries[threadIdx.x] : ~(u64)0;
+    int rank      = 0;
+#pragma unroll 4
+    for (int i = 0; i < count; ++i) rank += box.entries[i] > own;
+    if ((int)threadIdx.x < count && rank < a.k) write(rank, own);
+    return;
   }
   int size = 1;
   while (size < count) size <<= 1;
   for (int i = count + (int)threadIdx.x; i < size; i += THREADS) box.entries[i] = 0;
   sort_entries<THREADS>(box.entries, size);
-  for (int j = threadIdx.x; j < a.k; j += THREADS) {
-    const u32 i       = entry_index(box.entries[j]);
-    const int64_t out = (int64_t)r * a.k + j;
-    static_cast<T*>(a.values)[out] = row[i];
-    a.indices[out]                 = (int32_t)i;
-  }
+  for (int j = threadIdx.x; j < a.k; j += THREADS) write(j, box.entries[j]);
 }
 
-template <class T, int THREADS>
+template <class T, int W, int NV>
 int launch_rows(const TopKArgs& a, hipStream_t st)
 {
-  const dim3 grid((unsigned)a.n_rows), block(THREADS);
+  const dim3 grid((unsigned)a.n_rows), block(64 * W);
   if (a.lse != nullptr)
-    hipLaunchKernelGGL((top_k_kernel<T, THREADS, true>), grid, block, 0, st, a);
+    hipLaunchKernelGGL((top_k_kernel<T, W, NV, true>), grid, block, 0, st, a);
   else
-    hipLaunchKernelGGL((top_k_kernel<T, THREADS, false>), grid, block, 0, st, a);
+    hipLaunchKernelGGL((top_k_kernel<T, W, NV, false>), grid, block, 0, st, a);
   return hipGetLastError() == hipSuccess ? RMI_OK : RMI_ERR_LAUNCH;
 }
 
 template <class T>
 int launch(const TopKArgs& a, hipStream_t st)
 {
-  // A workgroup of 256 threads sets its threshold from 1024 vectors' maxima, which is sharp while k is
-  // a quarter of that; few long rows want all the loads that one CU can have in flight.
-  const bool few = a.n_rows <= 512 && (int64_t)a.n_cols * (int)sizeof(T) >= 32768;
-  if (a.k > 512 || few) return launch_rows<T, 1024>(a, st);
-  if (a.k > 256) return launch_rows<T, 512>(a, st);
-  return launch_rows<T, 256>(a, st);
+  const int64_t vectors = (int64_t)a.n_cols / In<T>::VEC;
+  // A workgroup of W waves sets its threshold from 256 W maxima, which is sharp while k is a quarter of
+  // that; few long rows want all the loads that one CU can have in flight.
+  const bool few = a.n_rows <= 512 && vectors >= 2048;
+  if (a.k > 512 || few) return launch_rows<T, 16, 4>(a, st);
+  if (a.k > 256) return launch_rows<T, 8, 8>(a, st);
+  if (vectors > 2048) return launch_rows<T, 4, 16>(a, st);
+  return vectors > 1024 ? launch_rows<T, 4, 8>(a, st) : launch_rows<T, 4, 4>(a, st);
 }
 
 }  // namespace

@@ -122,6 +122,25 @@ def test_top_k_strides_and_offsets(gpu, dtype, pad, offset):
         assert (memory == before).all()
 
 
+@pytest.mark.parametrize("dtype,quiet", [("f32", 0x7f800001), ("bf16", 0x7f81), ("f16", 0x7c01)])
+@pytest.mark.parametrize("n", [12, 300, 5000, 70000])
+def test_signalling_nans_rank_last_too(gpu, dtype, quiet, n):
+    """NaN bit patterns that no arithmetic makes, among the largest elements of their vectors."""
+    import torch
+    rng = np.random.default_rng(n)
+    view, _ = _put(rng.normal(0, 1, (4, n)), dtype)
+    bits = view.view(torch.int32 if dtype == "f32" else torch.int16)
+    places = torch.as_tensor(rng.random((4, n)) < 0.2).cuda()
+    places[3, :] = True
+    places[3, 5] = False
+    bits[places] = quiet
+    for k in (1, 10, min(n, 200)):
+        _check_top_k(view, k)
+    u = rng.random(4)
+    _check_sample(view, u)
+    _check_sample(view, u, top_k=np.full(4, 20), top_p=np.full(4, 0.9))
+
+
 def test_top_k_offsets_past_32_bits(gpu):
     """Rows that start more than 2^32 elements into the matrix."""
     import torch
