@@ -290,21 +290,32 @@ __device__ __forceinline__ u32 mask_bits(const u32* allowed, int i, int words)
   return __builtin_amdgcn_alignbit(hi, lo, (u32)i & 31u);
 }
 
-// The largest t, in the upper 16 bits of a key, such that at least `need` of the wave's 64 G keys are
-// t or more; 0 if there are fewer.  Sixteen steps of G comparisons each, counted over the lanes by
-// scalar instructions: no trip to LDS.
+// A t such that at least `need` of the wave's 64 G keys are t or more, and about as many as that: the
+// largest with zeros below bit 16; 0 if there are fewer such keys than zero.  A step compares the G keys
+// and counts over the lanes by scalar instructions, without a trip to LDS.  What is wanted mostly lies within
+// two powers of two (2^24 keys) of the largest key: nine steps then do, sixteen otherwise.
 template <int G>
 __device__ __forceinline__ u32 wave_rank(const u32 (&key)[G], int need)
 {
-  u32 t = 0;
-#pragma unroll 1
-  for (u32 bit = 0x80000000u; bit >= 0x10000u; bit >>= 1) {
-    const u32 trial = t | bit;
-    int have        = 0;
+  auto have = [&](u32 t) {
+    int n = 0;
 #pragma unroll
-    for (int g = 0; g < G; ++g) have += __popcll(__ballot(key[g] >= trial));
-    if (have >= need) t = trial;
+    for (int g = 0; g < G; ++g) n += __popcll(__ballot(key[g] >= t));
+    return n;
+  };
+  u32 top = key[0];
+#pragma unroll
+  for (int g = 1; g < G; ++g) top = top > key[g] ? top : key[g];
+  top       = __builtin_amdgcn_readfirstlane(wave_all(top, MaxF{}));
+  u32 t     = top > 0x01000000u ? (top - 0x01000000u) & 0xffff0000u : 0u;
+  u32 first = 0x00800000u;  // t + 2^24 is above all keys but for the bits below bit 16
+  if (t == 0 || have(t) < need) {
+    t     = 0;
+    first = 0x80000000u;
   }
+#pragma unroll 1
+  for (u32 bit = first; bit >= 0x10000u; bit >>= 1)
+    if (have(t + bit) >= need) t += bit;
   return t;
 }
 
@@ -524,18 +535,14 @@ __device__ __forceinline__ Found stream_candidates(const T* row, int n, int k, c
     return __builtin_nontemporal_load(
       reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(body + (int64_t)first * VEC) + off));
   };
-  // The elements of a vector; what does not count, or lies behind the last vector, is -inf.
-  auto unpack = [&](const u32x4& w, int v, float(&x)[VEC], bool whole) {
+  // The elements of a vector; what does not count is -inf.
+  auto unpack = [&](const u32x4& w, int v, float(&x)[VEC]) {
     static_for<VEC>([&](auto j) { x[j] = (float)In<T>::template get<j>(w); });
     if constexpr (LOOK == Look::kMasked) {
       const int at   = v < last ? v : last;
       const u32 bits = mask_bits(allowed, vs.head + at * VEC, words);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) x[j] = (bits >> j) & 1u ? x[j] : -kInf;
-    }
-    if (!whole && v >= vs.nv) {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) x[j] = -kInf;
     }
   };
   auto put = [&](float x, int i) {
@@ -565,10 +572,16 @@ __device__ __forceinline__ Found stream_candidates(const T* row, int n, int k, c
       }
       float x[PAIR][VEC];
 #pragma unroll
-      for (int p = 0; p < PAIR; ++p) {
-        unpack(now[i + p], first + (i + p) * THREADS + tid, x[p], whole);
-        m[i + p] = max_of(x[p]);
+      for (int p = 0; p < PAIR; ++p) unpack(now[i + p], first + (i + p) * THREADS + tid, x[p]);
+      if (!whole && first + (i + PAIR) * THREADS > vs.nv) {  // the same for all lanes
+#pragma unroll
+        for (int p = 0; p < PAIR; ++p)
+#pragma unroll
+          for (int j = 0; j < VEC; ++j)
+            x[p][j] = first + (i + p) * THREADS + tid < vs.nv ? x[p][j] : -kInf;
       }
+#pragma unroll
+      for (int p = 0; p < PAIR; ++p) m[i + p] = max_of(x[p]);
       const float most = max3(m[i], m[i + 1], -kInf);
       seen_max         = max3(seen_max, most, most);
       if constexpr (SUM) {
@@ -611,16 +624,15 @@ __device__ __forceinline__ Found stream_candidates(const T* row, int n, int k, c
     }
   };
   auto first_threshold = [&]() {
-    u32 key[5];
-    key[4] = ext_on && ext > -kInf ? key32(ext) : 0u;
+    u32 key[4];
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      float o = -kInf;
+      float o = g == 0 ? ext : -kInf;  // the element outside the vectors counts with the first
 #pragma unroll
       for (int i = g * GROUP; i < (g + 1) * GROUP; ++i) o = max3(o, m[i], m[i]);
       key[g] = o > -kInf ? key32(o) : 0u;
     }
-    tau = wave_rank<5>(key, (k + W - 1) / W);
+    tau = wave_rank<4>(key, (k + W - 1) / W);
     if ((tid & 63) == 0) box.word[tid >> 6] = tau;
     __syncthreads();
 #pragma unroll

@@ -116,6 +116,7 @@ __global__ __launch_bounds__(64 * W, 4) void top_k_kernel(TopKArgs a)
   if (count <= THREADS) {
     // a thread per candidate counts those that rank before it: no barrier, and every lane reads the
     // same place in LDS
+    if ((int)(threadIdx.x & ~63u) >= count) return;
     const u64 own = (int)threadIdx.x < count ? box.entries[threadIdx.x] : ~(u64)0;
     int rank      = 0;
 #pragma unroll 4
