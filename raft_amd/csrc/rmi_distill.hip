@@ -8,6 +8,8 @@
 #include "rmi_normalize.hpp"
 
 namespace rmi {
+int cu_count();  // rmi_api.hip
+
 namespace logits {
 namespace {
 
@@ -25,6 +27,7 @@ struct DistillArgs {
   int t_dtype;
   float c;           // log2(e) / T
   double inv_t, scale;
+  double ln2_t;      // ln(2) T
 };
 
 __device__ __forceinline__ double teacher(const DistillArgs& a, int64_t at)
@@ -36,145 +39,547 @@ __device__ __forceinline__ double teacher(const DistillArgs& a, int64_t at)
   }
 }
 
-// A running (max, sum of exponentials) of part of a row.
-struct MaxSum {
-  float m = -kInf;
-  float s = 0;
-};
-__device__ __forceinline__ float finite_or_zero(float m) { return fabsf(m) < kInf ? m : 0.0f; }
-
-// One workgroup per row: the running maximum and sum of the row (or the caller's), the teacher's
-// probabilities in 64 bits, the loss, and a second sweep that writes the gradient.  The teacher's
-// entries are written over the dense gradient after a barrier.
-template <class T, int THREADS, bool FORWARD, bool GRAD>
-__global__ __launch_bounds__(THREADS) void distill_kernel(DistillArgs a)
+// VEC values as one 16-byte vector, rounded to nearest even.
+template <class T>
+__device__ __forceinline__ u32x4 pack(const float (&y)[In<T>::VEC])
 {
-  constexpr int W   = THREADS / 64;
-  constexpr int VEC = In<T>::VEC;
-  __shared__ double p_of[RMI_DISTILL_MAX];
-  __shared__ int32_t i_of[RMI_DISTILL_MAX];
-  __shared__ float z_of[RMI_DISTILL_MAX];
-  __shared__ double box[W];
-  const int r  = blockIdx.x;
-  const T* row = static_cast<const T*>(a.z) + (int64_t)r * a.ld;
-  const int n  = a.n_cols;
+  u32x4 w;
+  if constexpr (std::is_same_v<T, float>) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = as_u32(y[j]);
+  } else if constexpr (std::is_same_v<T, bf16_t>) {
+    typedef __bf16 pair __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const pair p = {(__bf16)y[2 * j], (__bf16)y[2 * j + 1]};  // one v_cvt_pk_bf16_f32
+      w[j]         = __builtin_bit_cast(u32, p);
+    }
+  } else {
+    typedef _Float16 pair __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const pair p = {(_Float16)y[2 * j], (_Float16)y[2 * j + 1]};
+      w[j]         = __builtin_bit_cast(u32, p);
+    }
+  }
+  return w;
+}
 
-  // the teacher's entries; the student's logits at their places are read before any is overwritten
-  double best = -kInf;
-  for (int j = threadIdx.x; j < a.k; j += THREADS) {
-    const int64_t at = (int64_t)r * a.k + j;
+// What the first wave of a workgroup keeps in LDS of a row's teacher; `slot` is a hash table that finds
+// out whether a token is listed twice.
+struct TeacherBox {
+  double* p;
+  float* z;
+  int* index;
+  int* slot;
+  int slots;  // a power of two, at least 2 k
+  __device__ __forceinline__ TeacherBox(void* lds, int k, int slots_) : slots(slots_)
+  {
+    p     = static_cast<double*>(lds);
+    z     = reinterpret_cast<float*>(p + k);
+    index = reinterpret_cast<int*>(z + k);
+    slot  = index + k;
+  }
+  static int slots_of(int k)
+  {
+    int n = 64;
+    while (n < 2 * k) n *= 2;
+    return n;
+  }
+  static size_t bytes(int k) { return (size_t)k * 16 + (size_t)slots_of(k) * 4; }
+};
+
+// The teacher of one row, by one wave, in 64 bits: p_j in box.p (0 for unused entries), the
+// student's logits at its places in box.z, read before any of them is overwritten.  Returns their
+// mass; `twice` tells whether a token is listed more than once.
+template <class T>
+__device__ __forceinline__ double teacher_in(const DistillArgs& a, int64_t r, const T* row, TeacherBox& box, bool& twice)
+{
+  const int lane = (int)(threadIdx.x & 63);
+  double best    = -kInf;
+  for (int j = lane; j < box.slots; j += 64) box.slot[j] = -1;
+  for (int j = lane; j < a.k; j += 64) {
+    const int64_t at = r * a.k + j;
     int i            = a.index[at];
-    i                = i >= 0 && i < n ? i : -1;
+    i                = i >= 0 && i < a.n_cols ? i : -1;
     const double t   = teacher(a, at) * a.inv_t;
-    i_of[j]          = i;
-    p_of[j]          = t;
-    z_of[j]          = i >= 0 ? widen(row + i) : 0.0f;
+    box.index[j]     = i;
+    box.p[j]         = t;
+    box.z[j]         = i >= 0 ? widen(row + i) : 0.0f;
     if (i >= 0) best = fmax(best, t);
   }
   double norm;
   if (a.t_lse != nullptr) {
     norm = (double)a.t_lse[r];
   } else {
-    best         = block_all<W>(best, [](double x, double y) { return fmax(x, y); }, box);
+    best             = wave_all(best, [](double x, double y) { return fmax(x, y); });
     const double ref = best > -kInf ? best : 0.0;
-    double sum   = 0;
-    for (int j = threadIdx.x; j < a.k; j += THREADS)
-      if (i_of[j] >= 0) sum += exp(p_of[j] - ref);
-    sum  = block_all<W>(sum, AddF{}, box);
-    norm = ref + log(sum);
+    double sum       = 0;
+    for (int j = lane; j < a.k; j += 64)
+      if (box.index[j] >= 0) sum += exp(box.p[j] - ref);
+    norm = ref + log(wave_all(sum, AddF{}));
   }
-
-  double m, log_s;
-  float s;
-  if constexpr (FORWARD) {
-    MaxSum ms;
-    sweep<T, THREADS>(row, n, [&](float x, int) {
-      if (x > ms.m) {
-        const float ref = finite_or_zero(x);
-        ms.s *= __builtin_amdgcn_exp2f((ms.m - ref) * a.c);
-        ms.m = x;
-      }
-      ms.s += __builtin_amdgcn_exp2f((x - finite_or_zero(ms.m)) * a.c);
-    });
-    const float top = block_all<W>(ms.m, MaxF{}, reinterpret_cast<float*>(box));
-    const float ref = finite_or_zero(top);
-    const float own = ms.m > -kInf ? ms.s * __builtin_amdgcn_exp2f((ms.m - ref) * a.c) : ms.s;
-    const double all = block_all<W>((double)own, AddF{}, box);
-    m     = (double)ref;
-    log_s = log(all);
-    s     = (float)all;
-    if (a.stats != nullptr && threadIdx.x == 0) {
-      a.stats[2 * (int64_t)r]     = all == 0 ? -kInf : ref;
-      a.stats[2 * (int64_t)r + 1] = (float)log_s;
-    }
-  } else {
-    m     = (double)finite_or_zero(a.stats[2 * (int64_t)r]);
-    log_s = (double)a.stats[2 * (int64_t)r + 1];
-    s     = (float)exp(log_s);
-  }
-
-  double loss = 0, mass = 0;
-  for (int j = threadIdx.x; j < a.k; j += THREADS) {
-    double p = 0;
-    if (i_of[j] >= 0 && norm != -kInf) {
-      const double log_p = p_of[j] - norm;
-      p                  = exp(log_p);
-      if (p != 0) loss += p * (log_p - (((double)z_of[j] - m) * a.inv_t - log_s));
-    }
-    p_of[j] = p;
+  double mass = 0;
+  bool again  = false;
+  for (int j = lane; j < a.k; j += 64) {
+    const int i    = box.index[j];
+    const double p = i >= 0 && norm != -kInf ? exp(box.p[j] - norm) : 0.0;
+    box.p[j]       = p;
     mass += p;
+    if (i >= 0) {  // at most half of the table is taken, so every search ends
+      int h = (int)((u32)i * 2654435769u) & (box.slots - 1);
+      for (;;) {
+        const int was = atomicCAS(&box.slot[h], -1, i);
+        if (was == -1) break;
+        if (was == i) {
+          again = true;
+          break;
+        }
+        h = (h + 1) & (box.slots - 1);
+      }
+    }
   }
+  twice = __ballot(again) != 0;
+  return wave_all(mass, AddF{});
+}
+
+// The loss of a row, by the same wave: sum_j p_j (log p_j - (z_j - m) / T + log s).
+__device__ __forceinline__ double loss_of(const DistillArgs& a, const TeacherBox& box, double m, double log_s)
+{
+  double loss = 0;
+  for (int j = (int)(threadIdx.x & 63); j < a.k; j += 64) {
+    const double p = box.p[j];
+    if (p != 0) loss += p * (log(p) - (((double)box.z[j] - m) * a.inv_t - log_s));
+  }
+  return wave_all(loss, AddF{});
+}
+
+__device__ __forceinline__ void write_loss(const DistillArgs& a, const TeacherBox& box, int64_t r, float top, double m,
+                                           double all)
+{
+  const double log_s = log(all);
+  const double loss  = loss_of(a, box, m, log_s);
+  if ((threadIdx.x & 63) != 0) return;
+  a.loss[r] = (float)(loss * a.scale);
+  if (a.stats != nullptr) {
+    const double ref = (double)Running::ref(top);
+    a.stats[2 * r]     = all == 0 ? -kInf : Running::ref(top);
+    a.stats[2 * r + 1] = (float)(log_s + (m - ref) * a.inv_t);
+  }
+}
+
+// The gradient at the listed tokens, over the dense part that has been written there.
+template <class T>
+__device__ __forceinline__ void patch(const DistillArgs& a, const TeacherBox& box, T* out, double c, double mass, double m,
+                                      double s, bool twice)
+{
+  for (int j = (int)(threadIdx.x & 63); j < a.k; j += 64) {
+    const int i = box.index[j];
+    if (i < 0) continue;
+    double p = box.p[j];
+    if (twice) {  // every entry of a token writes the whole sum
+      p = 0;
+      for (int o = 0; o < a.k; ++o)
+        if (box.index[o] == i) p += box.p[o];
+    }
+    const double q = s == 0 ? 0.0 : exp(((double)box.z[j] - m) * a.inv_t) / s;
+    Put<T>::st(out + i, (float)(c * (mass * q - p)));
+  }
+}
+
+// The sum of exponentials of one thread's elements, two vectors at a time, against the largest of its
+// first two vectors: no maxima after that, which are a third of the instructions.  Any reference gives the
+// sum as long as it neither overflows nor sinks: what a thread's elements say about that is seen in the sum
+// itself, which is at least 1 with a reference out of its own elements.  If it is not, or is not finite, or
+// the reference is too large for one fused step, the thread goes over its elements again and raises the
+// reference as it goes (`again`).
+struct Guess {
+  Running run;
+  template <int V>
+  __device__ __forceinline__ void first(const float (&x)[2][V], float ext, float c)
+  {
+    const float m = max3(max_of(x[0]), max_of(x[1]), ext);
+    run.m         = fabsf(m) < Running::kLarge ? m : 0.0f;
+    run.r         = run.m * c;
+  }
+  template <int V>
+  __device__ __forceinline__ void add(const float (&x)[2][V], float c)
+  {
+    float t[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) t[j & 1] += __builtin_amdgcn_exp2f(fmaf(x[i][j], c, -run.r));
+    run.s += t[0] + t[1];
+  }
+  __device__ __forceinline__ bool doubtful() const { return !(run.s >= 0.5f && run.s < kInf); }
+};
+
+// dense part of the gradient: f exp((x - m) / T), f = c P / s
+// Results of 16 bits take the factor into the exponent: exp2(x c - r + log2 |f|) is off by some 2^-19, which
+// their own rounding hides, and saves a multiplication per element; fp32 results multiply.
+template <class T>
+struct Dense {
+  static constexpr bool kFold = sizeof(T) == 2;
+  float f, r, ref, c;
+  u32 sign;
+  bool large, zero;
+  __device__ __forceinline__ Dense(float top, float c_, double factor, double mass, double s) : c(c_)
+  {
+    ref   = Running::ref(top);
+    r     = ref * c;
+    large = !(fabsf(top) < Running::kLarge);
+    // a row without a finite logit has q = 0 everywhere; without a teacher its gradient is zero
+    zero = mass == 0;
+    f    = s == 0 || zero ? 0.0f : (float)(factor * mass) / (float)s;
+    sign = 0;
+    if (kFold && !large) {
+      sign = f < 0 ? 0x80008000u : 0u;
+      r -= __builtin_amdgcn_logf(fabsf(f));  // f = 0: exp2(-inf) = 0
+    }
+  }
+  __device__ __forceinline__ u32x4 operator()(const u32x4& w) const
+  {
+    constexpr int VEC = In<T>::VEC;
+    if (zero) return u32x4{0, 0, 0, 0};
+    float x[VEC];
+    static_for<VEC>([&](auto j) { x[j] = (float)In<T>::template get<j>(w); });
+    if (large) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) x[j] = f * __builtin_amdgcn_exp2f((x[j] - ref) * c);
+      return pack<T>(x);
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      x[j] = __builtin_amdgcn_exp2f(fmaf(x[j], c, -r));
+      if (!kFold) x[j] *= f;
+    }
+    u32x4 y = pack<T>(x);
+    if constexpr (kFold) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[j] ^= sign;
+    }
+    return y;
+  }
+  __device__ __forceinline__ float one(float x) const
+  {
+    if (zero) return 0.0f;
+    if (large) return f * __builtin_amdgcn_exp2f((x - ref) * c);
+    x = __builtin_amdgcn_exp2f(fmaf(x, c, -r));
+    return kFold ? (sign != 0 ? -x : x) : x * f;
+  }
+};
+
+// A sum of exponentials that belongs to the maximum m, against the maximum `top` of all.
+__device__ __forceinline__ double against(float m, double sum, float top, float c)
+{
+  if (!(m > -kInf)) return sum;  // nothing, or NaN alone
+  const float q = Running::ref(top) * c;
+  return sum * (double)(fabsf(top) < Running::kLarge && fabsf(m) < Running::kLarge
+                          ? __builtin_amdgcn_exp2f(m * c - q)
+                          : __builtin_amdgcn_exp2f((m - Running::ref(top)) * c));
+}
+// A wave's maximum and sum into LDS.
+__device__ __forceinline__ void share(const Running& run, float c, float* max, double* sum)
+{
+  const float m  = wave_all(run.m, MaxF{});
+  const double s = wave_all(run.against(m, c), AddF{});
+  if ((threadIdx.x & 63) == 0) {
+    max[threadIdx.x >> 6] = m;
+    sum[threadIdx.x >> 6] = s;
+  }
+}
+// What share() left there, as one: lane w of every wave takes wave w's.
+template <int W>
+__device__ __forceinline__ void joined(const float* max, const double* sum, float c, float& top, double& all)
+{
+  const int lane = (int)(threadIdx.x & 63);
+  float m        = lane < W ? max[lane] : -kInf;
+  double s       = lane < W ? sum[lane] : 0.0;
+  top            = wave_all(m, MaxF{});
+  all            = wave_all(against(m, s, top, c), AddF{});
+}
+// What the sum's logarithm belongs to: fl(m c), as a value in units of the logits.
+__device__ __forceinline__ double m_of(float top, const DistillArgs& a)
+{
+  return fabsf(top) < Running::kLarge ? (double)(Running::ref(top) * a.c) * a.ln2_t : (double)Running::ref(top);
+}
+__device__ __forceinline__ double factor_of(const DistillArgs& a, int64_t r)
+{
+  return (a.row_grad != nullptr ? (double)a.row_grad[r] : 1.0) * a.scale * a.inv_t;
+}
+
+// Loss and gradient of rows that fit into the registers of a workgroup (NV vectors a thread): a row is
+// read once and written once.  The first wave does the teacher's part before its own share of the row, and
+// the rest of it when its registers are free again.
+template <class T, int W, int NV, bool STREAM>
+__global__ __launch_bounds__(64 * W, NV > 8 ? 4 : 8) void distill_rows_kernel(DistillArgs a, int slots)
+{
+  constexpr int THREADS = 64 * W;
+  constexpr int VEC     = In<T>::VEC;
+  extern __shared__ double lds[];
+  __shared__ float max[W];
+  __shared__ double sum[W];
+  __shared__ double mass_box;
+  maxima_ignore_nan();
+  TeacherBox box(lds, a.k, slots);
+  const int tid   = (int)threadIdx.x;
+  const int n     = a.n_cols;
+  const bool lead = tid < 64;
+  const int r     = (int)blockIdx.x;
+  const T* row    = static_cast<const T*>(a.z) + (int64_t)r * a.ld;
+  const Vectors<T> vs(row, n);
+  bool twice = false;
+  if (lead) {
+    const double mass = teacher_in(a, r, row, box, twice);
+    if (tid == 0) mass_box = mass;
+  }
+  u32x4 now[NV];
+  if (vs.nv > 0) {
+    const char* body = reinterpret_cast<const char*>(row + vs.head);
+    const u32 room   = (u32)(vs.nv - 1) * 16u;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      u32 off = (u32)(i * THREADS + tid) * 16u;
+      off     = off < room ? off : room;
+      now[i]  = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(body + off));
+    }
+  }
+  const int ext_i = vs.extra(n);
+  const float ext = ext_i >= 0 ? widen(row + ext_i) : -kInf;
+  auto pair = [&](int i, float(&x)[2][VEC]) {
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+      static_for<VEC>([&](auto j) { x[p][j] = (float)In<T>::template get<j>(now[i + p]); });
+    if ((i + 2) * THREADS > vs.nv) {  // behind the last vector: -inf
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) x[p][j] = (i + p) * THREADS + tid < vs.nv ? x[p][j] : -kInf;
+    }
+  };
+  Guess sums;
+#pragma unroll
+  for (int i = 0; i < NV; i += 2) {
+    if (i > 0 && i * THREADS >= vs.nv) continue;
+    float x[2][VEC];
+    pair(i, x);
+    if (i == 0) sums.first(x, ext, a.c);
+    sums.add(x, a.c);
+  }
+  sums.run.s += __builtin_amdgcn_exp2f(fmaf(ext, a.c, -sums.run.r));
+  // the vectors stay packed: without this the compiler keeps the unpacked elements of the first pass for
+  // the next ones, twice the registers of a 16-bit type
+#pragma unroll
+  for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(now[i]));
+  if (sums.doubtful()) {
+    sums.run = Running{};
+    const float one[1][1] = {{ext}};
+    sums.run.raise(ext, a.c);
+    sums.run.add(one, a.c);
+#pragma unroll
+    for (int i = 0; i < NV; i += 2) {
+      if (i * THREADS >= vs.nv) continue;
+      float x[2][VEC];
+      pair(i, x);
+      sums.run.raise(max3(max_of(x[0]), max_of(x[1]), -kInf), a.c);
+      sums.run.add(x, a.c);
+    }
+  }
+  const Running& run = sums.run;
+  share(run, a.c, max, sum);
+  __syncthreads();
+  float top;
+  double all;
+  joined<W>(max, sum, a.c, top, all);
+  const double mass = mass_box;
+  const double c    = factor_of(a, r);
+  T* out            = static_cast<T*>(a.grad) + (int64_t)r * a.ld_grad;
+  const Dense<T> dense(top, a.c, c, mass, all);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(now[i]));
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (i * THREADS >= vs.nv) continue;
+    const u32x4 y = dense(now[i]);
+    if (i * THREADS + tid < vs.nv) store16<STREAM>(out + vs.head + (int64_t)(i * THREADS + tid) * VEC, y);
+  }
+  if (ext_i >= 0) {
+    Put<T>::st(out + ext_i, dense.one(ext));
+  }
+  __syncthreads();  // the dense part is written before the listed tokens'
+  if (lead) {
+    const double m = m_of(top, a);
+    write_loss(a, box, r, top, m, all);
+    if (mass != 0) patch(a, box, out, c, mass, m, all, twice);
+  }
+}
+
+// One workgroup per row that is streamed: for its sum of exponentials (FORWARD), and for the gradient
+// (GRAD), which reads the row a second time if both are asked for.
+template <class T, int W, bool FORWARD, bool GRAD, bool STREAM>
+__global__ __launch_bounds__(64 * W, 4) void distill_stream_kernel(DistillArgs a, int slots)
+{
+  constexpr int THREADS = 64 * W;
+  constexpr int VEC     = In<T>::VEC;
+  constexpr int NV      = 4;
+  extern __shared__ double lds[];
+  __shared__ float max[W];
+  __shared__ double sum[W];
+  __shared__ double mass_box;
+  maxima_ignore_nan();
+  TeacherBox box(lds, a.k, slots);
+  const int tid   = (int)threadIdx.x;
+  const int n     = a.n_cols;
+  const bool lead = tid < 64;
+  const int r     = (int)blockIdx.x;
+  const T* row    = static_cast<const T*>(a.z) + (int64_t)r * a.ld;
+  const Vectors<T> vs(row, n);
+  const T* body   = row + vs.head;
+  const int last  = vs.nv > 0 ? vs.nv - 1 : 0;
+  constexpr int BATCH = THREADS * NV;
+  auto fetch = [&](int first, int i, auto keep) {
+    const int left = last - first;
+    const u32 room = (u32)(left < BATCH ? left : BATCH) * 16u;
+    u32 off        = (u32)(i * THREADS + tid) * 16u;
+    off            = off < room ? off : room;
+    const u32x4* p = reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(body + (int64_t)first * VEC) + off);
+    // a row that is read again is kept in the caches
+    if constexpr (keep) return *p;
+    else return __builtin_nontemporal_load(p);
+  };
+  const int ext_i = vs.extra(n);
+  const float ext = ext_i >= 0 ? widen(row + ext_i) : -kInf;
+  bool twice      = false;
+  if (lead) {
+    const double mass = teacher_in(a, r, row, box, twice);
+    if (tid == 0) mass_box = mass;
+  }
+  float top;
+  double all, m;
   if constexpr (FORWARD) {
-    loss = block_all<W>(loss, AddF{}, box);
-    if (threadIdx.x == 0) a.loss[r] = (float)(loss * a.scale);
+    Running run;
+    {
+      const float one[1][1] = {{ext}};
+      run.raise(ext, a.c);
+      if (ext_i >= 0) run.add(one, a.c);
+    }
+    using keep = std::integral_constant<bool, GRAD>;
+    u32x4 now[NV];
+    auto take_in = [&](int first, bool whole) {
+#pragma unroll
+      for (int i = 0; i < NV; i += 2) {
+        if (!whole && first + i * THREADS >= vs.nv) continue;
+        float x[2][VEC];
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+          static_for<VEC>([&](auto j) { x[p][j] = (float)In<T>::template get<j>(now[i + p]); });
+        if (!whole && first + (i + 2) * THREADS > vs.nv) {
+#pragma unroll
+          for (int p = 0; p < 2; ++p)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) x[p][j] = first + (i + p) * THREADS + tid < vs.nv ? x[p][j] : -kInf;
+        }
+        // loaded again as soon as the vectors are taken out of the registers
+        if (whole) {
+          const int next = first + BATCH <= last ? first + BATCH : last;
+#pragma unroll
+          for (int p = 0; p < 2; ++p) now[i + p] = fetch(next, i + p, keep{});
+        }
+        run.raise(max3(max_of(x[0]), max_of(x[1]), -kInf), a.c);
+        run.add(x, a.c);
+      }
+    };
+    if (vs.nv > 0) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) now[i] = fetch(0, i, keep{});
+    }
+    int first = 0;
+    for (; first + BATCH <= vs.nv; first += BATCH) take_in(first, true);
+    if (first < vs.nv) take_in(first, false);
+    share(run, a.c, max, sum);
+    __syncthreads();
+    joined<W>(max, sum, a.c, top, all);
+    m = m_of(top, a);
+    if (lead) write_loss(a, box, r, top, m, all);
+  } else {
+    top = a.stats[2 * (int64_t)r];
+    m   = m_of(top, a);
+    // against fl(m c), as the terms are
+    all = exp((double)a.stats[2 * (int64_t)r + 1] + ((double)Running::ref(top) - m) * a.inv_t);
+    __syncthreads();
   }
   if constexpr (GRAD) {
-    mass           = block_all<W>(mass, AddF{}, box);
-    const double g = a.row_grad != nullptr ? (double)a.row_grad[r] : 1.0;
-    const double c = g * a.scale * a.inv_t;
-    // a row without a finite logit has q = 0 everywhere; without a teacher its gradient is zero
-    const double dense = mass == 0 ? 0.0 : (s == 0 ? 0.0 : c * mass / (double)s);
-    const float f      = (float)dense;
-    const float ref    = (float)m;
-    T* out             = static_cast<T*>(a.grad) + (int64_t)r * a.ld_grad;
-    const bool zero    = mass == 0;
-    const int nv       = n / VEC;
-    for (int v = threadIdx.x; v < nv; v += THREADS) {
-      const u32x4 w = load16c(row + (int64_t)v * VEC);
-      u32x4 y;
-      static_for<VEC>([&](auto j) {
-        const float x = (float)In<T>::template get<j>(w);
-        Put<T>::template at<j>(y, zero ? 0.0f : f * __builtin_amdgcn_exp2f((x - ref) * a.c));
-      });
-      store16<false>(out + (int64_t)v * VEC, y);
+    const double mass = mass_box;
+    const double c    = factor_of(a, r);
+    const Dense<T> dense(top, a.c, c, mass, all);
+    T* out = static_cast<T*>(a.grad) + (int64_t)r * a.ld_grad;
+    for (int first = 0; first < vs.nv; first += BATCH) {
+      u32x4 now[NV];
+#pragma unroll
+      for (int i = 0; i < NV; ++i) now[i] = fetch(first, i, std::false_type{});
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int v = first + i * THREADS + tid;
+        const u32x4 y = dense(now[i]);
+        if (v < vs.nv) store16<STREAM>(out + vs.head + (int64_t)v * VEC, y);
+      }
     }
-    for (int i = nv * VEC + threadIdx.x; i < n; i += THREADS)
-      Put<T>::st(out + i, zero ? 0.0f : f * __builtin_amdgcn_exp2f((widen(row + i) - ref) * a.c));
+    if (ext_i >= 0) {
+      Put<T>::st(out + ext_i, dense.one(ext));
+    }
     __syncthreads();
-    if (zero) return;
-    for (int j = threadIdx.x; j < a.k; j += THREADS) {
-      const int i = i_of[j];
-      if (i < 0) continue;
-      double p = 0;  // the same token may be listed more than once: every entry writes the whole sum
-      for (int o = 0; o < a.k; ++o)
-        if (i_of[o] == i) p += p_of[o];
-      const double q = s == 0 ? 0.0 : exp(((double)z_of[j] - m) * a.inv_t) / (double)s;
-      Put<T>::st(out + i, (float)(c * (mass * q - p)));
-    }
+    if (lead && !dense.zero) patch(a, box, out, c, mass, m, all, twice);
   }
+}
+
+template <class T, int W, int NV, bool STREAM>
+void launch_rows(const DistillArgs& a, int slots, size_t lds, hipStream_t st)
+{
+  hipLaunchKernelGGL((distill_rows_kernel<T, W, NV, STREAM>), dim3((unsigned)a.n_rows), dim3(64 * W), lds, st, a, slots);
+}
+
+template <class T, bool STREAM>
+int launch_as(const DistillArgs& a, hipStream_t st)
+{
+  const int slots       = TeacherBox::slots_of(a.k);
+  const size_t lds      = TeacherBox::bytes(a.k);
+  const int64_t vectors = (int64_t)a.n_cols / In<T>::VEC;
+  const dim3 grid((unsigned)a.n_rows);
+  const bool few = a.n_rows <= 512 && vectors >= 1024;
+  if (a.loss == nullptr) {
+    if (few)
+      hipLaunchKernelGGL((distill_stream_kernel<T, 16, false, true, STREAM>), grid, dim3(1024), lds, st, a, slots);
+    else
+      hipLaunchKernelGGL((distill_stream_kernel<T, 4, false, true, STREAM>), grid, dim3(256), lds, st, a, slots);
+  } else if (a.grad == nullptr) {
+    if (few)
+      hipLaunchKernelGGL((distill_stream_kernel<T, 16, true, false, STREAM>), grid, dim3(1024), lds, st, a, slots);
+    else
+      hipLaunchKernelGGL((distill_stream_kernel<T, 4, true, false, STREAM>), grid, dim3(256), lds, st, a, slots);
+  } else if (vectors > 16384) {
+    hipLaunchKernelGGL((distill_stream_kernel<T, 8, true, true, STREAM>), grid, dim3(512), lds, st, a, slots);
+  } else if (vectors > 8192) {
+    launch_rows<T, 16, 16, STREAM>(a, slots, lds, st);
+  } else if (vectors > 4096) {
+    launch_rows<T, 16, 8, STREAM>(a, slots, lds, st);
+  } else if (vectors > 2048 && !few) {
+    launch_rows<T, 8, 8, STREAM>(a, slots, lds, st);
+  } else if (vectors > 1024) {
+    launch_rows<T, 16, 4, STREAM>(a, slots, lds, st);
+  } else {
+    launch_rows<T, 4, 4, STREAM>(a, slots, lds, st);
+  }
+  return hipGetLastError() == hipSuccess ? RMI_OK : RMI_ERR_LAUNCH;
 }
 
 template <class T>
 int launch(const DistillArgs& a, hipStream_t st)
 {
-  const dim3 grid((unsigned)a.n_rows), block(256);
-  if (a.loss == nullptr)
-    hipLaunchKernelGGL((distill_kernel<T, 256, false, true>), grid, block, 0, st, a);
-  else if (a.grad != nullptr)
-    hipLaunchKernelGGL((distill_kernel<T, 256, true, true>), grid, block, 0, st, a);
-  else
-    hipLaunchKernelGGL((distill_kernel<T, 256, true, false>), grid, block, 0, st, a);
-  return hipGetLastError() == hipSuccess ? RMI_OK : RMI_ERR_LAUNCH;
+  // Stores past the caches pay where the gradient's vectors lie on 16-byte boundaries like the logits'.
+  const bool alike = ((reinterpret_cast<uintptr_t>(a.z) ^ reinterpret_cast<uintptr_t>(a.grad)) & 15) == 0 &&
+                     ((a.ld - a.ld_grad) * (int64_t)sizeof(T)) % 16 == 0;
+  return alike ? launch_as<T, true>(a, st) : launch_as<T, false>(a, st);
 }
 
 int run(int dtype, int t_dtype, int64_t n_rows, int64_t n_cols, int64_t ld, int64_t k, double temperature,
@@ -202,6 +607,7 @@ int run(int dtype, int t_dtype, int64_t n_rows, int64_t n_cols, int64_t ld, int6
   a.t_dtype = t_dtype;
   a.inv_t   = 1.0 / temperature;
   a.scale   = scale;
+  a.ln2_t   = kLn2 * temperature;
   a.c       = (float)(kLog2e / temperature);
   hipStream_t st = static_cast<hipStream_t>(stream);
   switch (dtype) {
