@@ -89,36 +89,45 @@ struct TeacherBox {
   static size_t bytes(int k) { return (size_t)k * 16 + (size_t)slots_of(k) * 4; }
 };
 
-// The teacher of one row, by one wave, in 64 bits: p_j in box.p (0 for unused entries), the
-// student's logits at its places in box.z, read before any of them is overwritten.  Returns their
-// mass; `twice` tells whether a token is listed more than once.
-template <class T>
-__device__ __forceinline__ double teacher_in(const DistillArgs& a, int64_t r, const T* row, TeacherBox& box, bool& twice)
+// A row's teacher, by one wave, in 64 bits: its entries in box.index (-1: not used) and box.p (t / T), and
+// the logarithm that its probabilities are taken against.
+__device__ __forceinline__ double teacher_norm(const DistillArgs& a, int64_t r, TeacherBox& box)
 {
-  const int lane = (int)(threadIdx.x & 63);
-  double best    = -kInf;
-  for (int j = lane; j < box.slots; j += 64) box.slot[j] = -1;
-  for (int j = lane; j < a.k; j += 64) {
+  double best = -kInf;
+  for (int j = (int)(threadIdx.x & 63); j < a.k; j += 64) {
     const int64_t at = r * a.k + j;
     int i            = a.index[at];
     i                = i >= 0 && i < a.n_cols ? i : -1;
     const double t   = teacher(a, at) * a.inv_t;
     box.index[j]     = i;
     box.p[j]         = t;
-    box.z[j]         = i >= 0 ? widen(row + i) : 0.0f;
     if (i >= 0) best = fmax(best, t);
   }
-  double norm;
-  if (a.t_lse != nullptr) {
-    norm = (double)a.t_lse[r];
-  } else {
-    best             = wave_all(best, [](double x, double y) { return fmax(x, y); });
-    const double ref = best > -kInf ? best : 0.0;
-    double sum       = 0;
-    for (int j = lane; j < a.k; j += 64)
-      if (box.index[j] >= 0) sum += exp(box.p[j] - ref);
-    norm = ref + log(wave_all(sum, AddF{}));
-  }
+  if (a.t_lse != nullptr) return (double)a.t_lse[r];
+  best             = wave_all(best, [](double x, double y) { return fmax(x, y); });
+  const double ref = best > -kInf ? best : 0.0;
+  double sum       = 0;
+  for (int j = (int)(threadIdx.x & 63); j < a.k; j += 64)
+    if (box.index[j] >= 0) sum += exp(box.p[j] - ref);
+  return ref + log(wave_all(sum, AddF{}));
+}
+
+// q of one logit, in 64 bits
+__device__ __forceinline__ double share_of(const DistillArgs& a, float z, double m, double s)
+{
+  return s == 0 ? 0.0 : exp(((double)z - m) * a.inv_t) / s;
+}
+
+// The teacher of one row, by one wave, in 64 bits: p_j in box.p (0 for unused entries), the
+// student's logits at its places in box.z, read before any of them is overwritten.  Returns their
+// mass; `twice` tells whether a token is listed more than once.
+template <class T>
+__device__ __forceinline__ double teacher_in(const DistillArgs& a, int64_t r, const T* row, TeacherBox& box, bool& twice)
+{
+  const int lane    = (int)(threadIdx.x & 63);
+  const double norm = teacher_norm(a, r, box);
+  for (int j = lane; j < box.slots; j += 64) box.slot[j] = -1;
+  for (int j = lane; j < a.k; j += 64) box.z[j] = box.index[j] >= 0 ? widen(row + box.index[j]) : 0.0f;
   double mass = 0;
   bool again  = false;
   for (int j = lane; j < a.k; j += 64) {
@@ -182,8 +191,7 @@ __device__ __forceinline__ void patch(const DistillArgs& a, const TeacherBox& bo
       for (int o = 0; o < a.k; ++o)
         if (box.index[o] == i) p += box.p[o];
     }
-    const double q = s == 0 ? 0.0 : exp(((double)box.z[j] - m) * a.inv_t) / s;
-    Put<T>::st(out + i, (float)(c * (mass * q - p)));
+    Put<T>::st(out + i, (float)(c * (mass * share_of(a, box.z[j], m, s) - p)));
   }
 }
 
@@ -312,7 +320,7 @@ __device__ __forceinline__ double factor_of(const DistillArgs& a, int64_t r)
 // Loss and gradient of rows that fit into the registers of a workgroup (NV vectors a thread): a row is
 // read once and written once.  The first wave does the teacher's part before its own share of the row, and
 // the rest of it when its registers are free again.
-template <class T, int W, int NV, bool STREAM>
+template <class T, int W, int NV>
 __global__ __launch_bounds__(64 * W, NV > 8 ? 4 : 8) void distill_rows_kernel(DistillArgs a, int slots)
 {
   constexpr int THREADS = 64 * W;
@@ -326,9 +334,11 @@ __global__ __launch_bounds__(64 * W, NV > 8 ? 4 : 8) void distill_rows_kernel(Di
   const int tid   = (int)threadIdx.x;
   const int n     = a.n_cols;
   const bool lead = tid < 64;
-  const int r     = (int)blockIdx.x;
-  const T* row    = static_cast<const T*>(a.z) + (int64_t)r * a.ld;
-  const Vectors<T> vs(row, n);
+  const int64_t r = block_of_grid();
+  if (r >= a.n_rows) return;
+  const T* row    = static_cast<const T*>(a.z) + r * a.ld;
+  T* out          = static_cast<T*>(a.grad) + r * a.ld_grad;
+  const Vectors<T, 128> vs(out, n);  // whole lines where the gradient is stored
   bool twice = false;
   if (lead) {
     const double mass = teacher_in(a, r, row, box, twice);
@@ -342,7 +352,7 @@ __global__ __launch_bounds__(64 * W, NV > 8 ? 4 : 8) void distill_rows_kernel(Di
     for (int i = 0; i < NV; ++i) {
       u32 off = (u32)(i * THREADS + tid) * 16u;
       off     = off < room ? off : room;
-      now[i]  = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(body + off));
+      now[i]  = load16(body + off);
     }
   }
   const int ext_i = vs.extra(n);
@@ -394,7 +404,6 @@ __global__ __launch_bounds__(64 * W, NV > 8 ? 4 : 8) void distill_rows_kernel(Di
   joined<W>(max, sum, a.c, top, all);
   const double mass = mass_box;
   const double c    = factor_of(a, r);
-  T* out            = static_cast<T*>(a.grad) + (int64_t)r * a.ld_grad;
   const Dense<T> dense(top, a.c, c, mass, all);
 #pragma unroll
   for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(now[i]));
@@ -402,7 +411,7 @@ __global__ __launch_bounds__(64 * W, NV > 8 ? 4 : 8) void distill_rows_kernel(Di
   for (int i = 0; i < NV; ++i) {
     if (i * THREADS >= vs.nv) continue;
     const u32x4 y = dense(now[i]);
-    if (i * THREADS + tid < vs.nv) store16<STREAM>(out + vs.head + (int64_t)(i * THREADS + tid) * VEC, y);
+    if (i * THREADS + tid < vs.nv) store16<true>(out + vs.head + (int64_t)(i * THREADS + tid) * VEC, y);
   }
   if (ext_i >= 0) {
     Put<T>::st(out + ext_i, dense.one(ext));
@@ -415,9 +424,90 @@ __global__ __launch_bounds__(64 * W, NV > 8 ? 4 : 8) void distill_rows_kernel(Di
   }
 }
 
-// One workgroup per row that is streamed: for its sum of exponentials (FORWARD), and for the gradient
-// (GRAD), which reads the row a second time if both are asked for.
-template <class T, int W, bool FORWARD, bool GRAD, bool STREAM>
+// The gradient from the statistics of an earlier forward pass: nothing joins a row's parts, so every
+// workgroup takes one piece of a row, NV vectors a thread, in the order of memory.  (A workgroup that walks
+// a whole row keeps a thousand rows open at once: 1000 x 50001 f32: 92 us against 77.)  Its first wave works the
+// teacher's probabilities out again and corrects the listed tokens that lie in the piece.
+template <class T, int W, int NV>
+__global__ __launch_bounds__(64 * W, 6) void distill_grad_kernel(DistillArgs a, int pieces)
+{
+  constexpr int THREADS = 64 * W;
+  constexpr int VEC     = In<T>::VEC;
+  extern __shared__ double lds[];
+  __shared__ double mass_box;
+  const int tid   = (int)threadIdx.x;
+  const int n     = a.n_cols;
+  const bool lead = tid < 64;
+  const int64_t r = block_of_grid() / pieces;
+  const int piece = (int)(block_of_grid() % pieces);
+  if (r >= a.n_rows) return;
+  const T* row    = static_cast<const T*>(a.z) + r * a.ld;
+  T* out          = static_cast<T*>(a.grad) + r * a.ld_grad;
+  const Vectors<T, 128> vs(out, n);  // whole lines where the gradient is stored
+  // vectors [from, to) of the row; the first piece also has the elements outside the vectors
+  const int per  = ((n / VEC + pieces - 1) / pieces + 63) & ~63;  // a wave's stores cover whole lines
+  const int from = min(piece * per, vs.nv);
+  const int to   = min(from + per, vs.nv);
+  u32x4 now[NV];
+  if (from < to) {
+    const char* body = reinterpret_cast<const char*>(row + vs.head + (int64_t)from * VEC);
+    const u32 room   = (u32)(to - from - 1) * 16u;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      u32 off = (u32)(i * THREADS + tid) * 16u;
+      off     = off < room ? off : room;
+      now[i]  = load16(body + off);
+    }
+  }
+  const int ext_i = piece == 0 ? vs.extra(n) : -1;
+  const float ext = ext_i >= 0 ? widen(row + ext_i) : -kInf;
+  const float top = a.stats[2 * r];
+  const double m  = m_of(top, a);
+  // against fl(m c), as the terms are
+  const double all = exp((double)a.stats[2 * r + 1] + ((double)Running::ref(top) - m) * a.inv_t);
+  TeacherBox box(lds, a.k, 0);
+  const int lo    = vs.head + from * VEC, hi = vs.head + to * VEC;
+  auto mine       = [&](int i) { return (i >= lo && i < hi) || (piece == 0 && i >= 0 && (i < vs.head || i >= vs.head + vs.nv * VEC)); };
+  if (lead) {
+    const double norm = teacher_norm(a, r, box);
+    double mass       = 0;
+    for (int j = tid; j < a.k; j += 64) {
+      const int i    = box.index[j];
+      const double p = i >= 0 && norm != -kInf ? exp(box.p[j] - norm) : 0.0;
+      box.p[j]       = p;
+      mass += p;
+      if (mine(i)) box.z[j] = widen(row + i);
+    }
+    mass = wave_all(mass, AddF{});
+    if (tid == 0) mass_box = mass;
+  }
+  __syncthreads();  // the logits at the listed tokens are read before any of the piece is overwritten
+  const double mass = mass_box;
+  const double c    = factor_of(a, r);
+  const Dense<T> dense(top, a.c, c, mass, all);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int v = from + i * THREADS + tid;
+    if (from + i * THREADS >= to) continue;
+    const u32x4 y = dense(now[i]);
+    if (v < to) store16<true>(out + vs.head + (int64_t)v * VEC, y);
+  }
+  if (ext_i >= 0) Put<T>::st(out + ext_i, dense.one(ext));
+  __syncthreads();  // the dense part is written before the listed tokens'
+  if (!lead || mass == 0) return;
+  for (int j = tid; j < a.k; j += 64) {
+    const int i = box.index[j];
+    if (!mine(i)) continue;
+    double p = 0;  // the same token may be listed more than once: every entry writes the whole sum
+    for (int o = 0; o < a.k; ++o)
+      if (box.index[o] == i) p += box.p[o];
+    Put<T>::st(out + i, (float)(c * (mass * share_of(a, box.z[j], m, all) - p)));
+  }
+}
+
+// One workgroup per row that is streamed, for the sum of its exponentials; if the gradient is wanted too,
+// the row, too long for a workgroup's registers, is read a second time.
+template <class T, int W, bool GRAD>
 __global__ __launch_bounds__(64 * W, 4) void distill_stream_kernel(DistillArgs a, int slots)
 {
   constexpr int THREADS = 64 * W;
@@ -432,9 +522,11 @@ __global__ __launch_bounds__(64 * W, 4) void distill_stream_kernel(DistillArgs a
   const int tid   = (int)threadIdx.x;
   const int n     = a.n_cols;
   const bool lead = tid < 64;
-  const int r     = (int)blockIdx.x;
-  const T* row    = static_cast<const T*>(a.z) + (int64_t)r * a.ld;
-  const Vectors<T> vs(row, n);
+  const int64_t r = block_of_grid();
+  if (r >= a.n_rows) return;
+  const T* row    = static_cast<const T*>(a.z) + r * a.ld;
+  T* out          = GRAD ? static_cast<T*>(a.grad) + r * a.ld_grad : nullptr;
+  const Vectors<T, GRAD ? 128 : 16> vs(GRAD ? out : row, n);  // whole lines where the gradient is stored
   const T* body   = row + vs.head;
   const int last  = vs.nv > 0 ? vs.nv - 1 : 0;
   constexpr int BATCH = THREADS * NV;
@@ -443,10 +535,10 @@ __global__ __launch_bounds__(64 * W, 4) void distill_stream_kernel(DistillArgs a
     const u32 room = (u32)(left < BATCH ? left : BATCH) * 16u;
     u32 off        = (u32)(i * THREADS + tid) * 16u;
     off            = off < room ? off : room;
-    const u32x4* p = reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(body + (int64_t)first * VEC) + off);
+    const char* p  = reinterpret_cast<const char*>(body + (int64_t)first * VEC) + off;
     // a row that is read again is kept in the caches
-    if constexpr (keep) return *p;
-    else return __builtin_nontemporal_load(p);
+    if constexpr (keep) return load16c(p);
+    else return load16(p);
   };
   const int ext_i = vs.extra(n);
   const float ext = ext_i >= 0 ? widen(row + ext_i) : -kInf;
@@ -456,8 +548,8 @@ __global__ __launch_bounds__(64 * W, 4) void distill_stream_kernel(DistillArgs a
     if (tid == 0) mass_box = mass;
   }
   float top;
-  double all, m;
-  if constexpr (FORWARD) {
+  double all;
+  {
     Running run;
     {
       const float one[1][1] = {{ext}};
@@ -500,29 +592,30 @@ __global__ __launch_bounds__(64 * W, 4) void distill_stream_kernel(DistillArgs a
     share(run, a.c, max, sum);
     __syncthreads();
     joined<W>(max, sum, a.c, top, all);
-    m = m_of(top, a);
-    if (lead) write_loss(a, box, r, top, m, all);
-  } else {
-    top = a.stats[2 * (int64_t)r];
-    m   = m_of(top, a);
-    // against fl(m c), as the terms are
-    all = exp((double)a.stats[2 * (int64_t)r + 1] + ((double)Running::ref(top) - m) * a.inv_t);
-    __syncthreads();
   }
+  const double m = m_of(top, a);
+  if (lead) write_loss(a, box, r, top, m, all);
   if constexpr (GRAD) {
     const double mass = mass_box;
     const double c    = factor_of(a, r);
     const Dense<T> dense(top, a.c, c, mass, all);
-    T* out = static_cast<T*>(a.grad) + (int64_t)r * a.ld_grad;
-    for (int first = 0; first < vs.nv; first += BATCH) {
-      u32x4 now[NV];
+    // The next batch is asked for before this one is stored: loads and stores are counted together, in
+    // order, so loads behind the stores would wait for them.
+    u32x4 now[NV], next[NV];
+    if (vs.nv > 0) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) now[i] = fetch(first, i, std::false_type{});
+      for (int i = 0; i < NV; ++i) now[i] = fetch(0, i, std::false_type{});
+    }
+    for (int first = 0; first < vs.nv; first += BATCH) {
+      const int ahead = first + BATCH <= last ? first + BATCH : last;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) next[i] = fetch(ahead, i, std::false_type{});
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int v = first + i * THREADS + tid;
         const u32x4 y = dense(now[i]);
-        if (v < vs.nv) store16<STREAM>(out + vs.head + (int64_t)v * VEC, y);
+        if (v < vs.nv) store16<true>(out + vs.head + (int64_t)v * VEC, y);
+        now[i] = next[i];
       }
     }
     if (ext_i >= 0) {
@@ -533,53 +626,44 @@ __global__ __launch_bounds__(64 * W, 4) void distill_stream_kernel(DistillArgs a
   }
 }
 
-template <class T, int W, int NV, bool STREAM>
+template <class T, int W, int NV>
 void launch_rows(const DistillArgs& a, int slots, size_t lds, hipStream_t st)
 {
-  hipLaunchKernelGGL((distill_rows_kernel<T, W, NV, STREAM>), dim3((unsigned)a.n_rows), dim3(64 * W), lds, st, a, slots);
-}
-
-template <class T, bool STREAM>
-int launch_as(const DistillArgs& a, hipStream_t st)
-{
-  const int slots       = TeacherBox::slots_of(a.k);
-  const size_t lds      = TeacherBox::bytes(a.k);
-  const int64_t vectors = (int64_t)a.n_cols / In<T>::VEC;
-  const dim3 grid((unsigned)a.n_rows);
-  const bool few = a.n_rows <= 512 && vectors >= 1024;
-  if (a.loss == nullptr) {
-    if (few)
-      hipLaunchKernelGGL((distill_stream_kernel<T, 16, false, true, STREAM>), grid, dim3(1024), lds, st, a, slots);
-    else
-      hipLaunchKernelGGL((distill_stream_kernel<T, 4, false, true, STREAM>), grid, dim3(256), lds, st, a, slots);
-  } else if (a.grad == nullptr) {
-    if (few)
-      hipLaunchKernelGGL((distill_stream_kernel<T, 16, true, false, STREAM>), grid, dim3(1024), lds, st, a, slots);
-    else
-      hipLaunchKernelGGL((distill_stream_kernel<T, 4, true, false, STREAM>), grid, dim3(256), lds, st, a, slots);
-  } else if (vectors > 16384) {
-    hipLaunchKernelGGL((distill_stream_kernel<T, 8, true, true, STREAM>), grid, dim3(512), lds, st, a, slots);
-  } else if (vectors > 8192) {
-    launch_rows<T, 16, 16, STREAM>(a, slots, lds, st);
-  } else if (vectors > 4096) {
-    launch_rows<T, 16, 8, STREAM>(a, slots, lds, st);
-  } else if (vectors > 2048 && !few) {
-    launch_rows<T, 8, 8, STREAM>(a, slots, lds, st);
-  } else if (vectors > 1024) {
-    launch_rows<T, 16, 4, STREAM>(a, slots, lds, st);
-  } else {
-    launch_rows<T, 4, 4, STREAM>(a, slots, lds, st);
-  }
-  return hipGetLastError() == hipSuccess ? RMI_OK : RMI_ERR_LAUNCH;
+  hipLaunchKernelGGL((distill_rows_kernel<T, W, NV>), grid_of(a.n_rows), dim3(64 * W), lds, st, a, slots);
 }
 
 template <class T>
 int launch(const DistillArgs& a, hipStream_t st)
 {
-  // Stores past the caches pay where the gradient's vectors lie on 16-byte boundaries like the logits'.
-  const bool alike = ((reinterpret_cast<uintptr_t>(a.z) ^ reinterpret_cast<uintptr_t>(a.grad)) & 15) == 0 &&
-                     ((a.ld - a.ld_grad) * (int64_t)sizeof(T)) % 16 == 0;
-  return alike ? launch_as<T, true>(a, st) : launch_as<T, false>(a, st);
+  const int slots       = TeacherBox::slots_of(a.k);
+  const size_t lds      = TeacherBox::bytes(a.k);
+  const int64_t vectors = (int64_t)a.n_cols / In<T>::VEC;
+  const dim3 grid = grid_of(a.n_rows);
+  const bool few = a.n_rows <= 512 && vectors >= 1024;
+  if (a.loss == nullptr) {
+    constexpr int W = 4, NV = 8;
+    const int pieces = vectors > 0 ? (int)((vectors + 64 * W * NV - 1) / (64 * W * NV)) : 1;
+    hipLaunchKernelGGL((distill_grad_kernel<T, W, NV>), grid_of(a.n_rows * (int64_t)pieces), dim3(64 * W), lds, st,
+                       a, pieces);
+  } else if (a.grad == nullptr) {
+    if (few)
+      hipLaunchKernelGGL((distill_stream_kernel<T, 16, false>), grid, dim3(1024), lds, st, a, slots);
+    else
+      hipLaunchKernelGGL((distill_stream_kernel<T, 4, false>), grid, dim3(256), lds, st, a, slots);
+  } else if (vectors > 16384) {
+    hipLaunchKernelGGL((distill_stream_kernel<T, 8, true>), grid, dim3(512), lds, st, a, slots);
+  } else if (vectors > 8192) {
+    launch_rows<T, 16, 16>(a, slots, lds, st);
+  } else if (vectors > 4096) {
+    launch_rows<T, 16, 8>(a, slots, lds, st);
+  } else if (vectors > 2048 && !few) {
+    launch_rows<T, 8, 8>(a, slots, lds, st);
+  } else if (vectors > 1024) {
+    launch_rows<T, 16, 4>(a, slots, lds, st);
+  } else {
+    launch_rows<T, 4, 4>(a, slots, lds, st);
+  }
+  return hipGetLastError() == hipSuccess ? RMI_OK : RMI_ERR_LAUNCH;
 }
 
 int run(int dtype, int t_dtype, int64_t n_rows, int64_t n_cols, int64_t ld, int64_t k, double temperature,

@@ -33,6 +33,15 @@ inline int check_shape(int64_t n_rows, int64_t n_cols, int64_t ld)
   return RMI_OK;
 }
 
+// Workgroups over rows (or pieces of them) as a grid of two dimensions: a launch holds fewer than 2^32
+// threads in each.
+inline dim3 grid_of(int64_t blocks)
+{
+  const int64_t x = blocks < (1 << 20) ? blocks : (1 << 20);
+  return dim3((unsigned)x, (unsigned)((blocks + x - 1) / x));
+}
+__device__ __forceinline__ int64_t block_of_grid() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+
 // ---- elements ---------------------------------------------------------------------------------
 
 // 16 bytes at any element's address, cached: rows are swept more than once.
@@ -262,22 +271,24 @@ __device__ Cut find_cut(const T* row, int n, u32 max_key, u64 target, F weigh, u
 
 // Where the aligned 16-byte vectors of a row lie: `head` elements come before them, `nv` vectors
 // follow, and what is left after them is shorter than a vector.  Reads of aligned vectors run at
-// the full rate whatever the row's length and stride are.
-template <class T>
+// the full rate whatever the row's length and stride are; rows that are written start their vectors on
+// a cache line (ALIGN = 128), so that no line is stored in parts.
+template <class T, int ALIGN = 16>
 struct Vectors {
   int head, nv;
   __device__ __forceinline__ Vectors(const T* row, int n)
   {
-    const int off = (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / (int)sizeof(T);
+    const int off = (int)((ALIGN - (reinterpret_cast<uintptr_t>(row) & (ALIGN - 1))) & (ALIGN - 1)) / (int)sizeof(T);
     head          = off < n ? off : n;
     nv            = (n - head) / In<T>::VEC;
   }
-  // The index of this thread's element outside the vectors, or -1 (there are at most 2 VEC - 2).
+  // The index of this thread's element outside the vectors, or -1 (there are fewer than ALIGN bytes in
+  // front and fewer than a vector behind).
   __device__ __forceinline__ int extra(int n) const
   {
     const int t = (int)threadIdx.x;
     const int i = t < head ? t : t + nv * In<T>::VEC;
-    return i < n && t < 2 * In<T>::VEC ? i : -1;
+    return i < n && t < ALIGN / (int)sizeof(T) + In<T>::VEC ? i : -1;
   }
 };
 

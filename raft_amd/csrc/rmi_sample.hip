@@ -45,10 +45,11 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleArgs a)
   __shared__ u64 bins[kBins + 2];
   __shared__ u64 box[W];
   __shared__ u64 found[2];
-  const int r        = blockIdx.x;
-  const T* row       = static_cast<const T*>(a.logits) + (int64_t)r * a.ld;
+  const int64_t r    = block_of_grid();
+  if (r >= a.n_rows) return;
+  const T* row       = static_cast<const T*>(a.logits) + r * a.ld;
   const int n        = a.n_cols;
-  const u32* allowed = a.allowed != nullptr ? a.allowed + (int64_t)r * a.ld_allowed : nullptr;
+  const u32* allowed = a.allowed != nullptr ? a.allowed + r * a.ld_allowed : nullptr;
   auto eligible      = [&](float x, int i) {
     return x > -kInf && (allowed == nullptr || ((allowed[i >> 5] >> (i & 31)) & 1u) != 0);
   };
@@ -176,7 +177,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleArgs a)
 template <class T>
 int launch(const SampleArgs& a, hipStream_t st)
 {
-  hipLaunchKernelGGL((sample_kernel<T, 1024>), dim3((unsigned)a.n_rows), dim3(1024), 0, st, a);
+  hipLaunchKernelGGL((sample_kernel<T, 1024>), grid_of(a.n_rows), dim3(1024), 0, st, a);
   return hipGetLastError() == hipSuccess ? RMI_OK : RMI_ERR_LAUNCH;
 }
 

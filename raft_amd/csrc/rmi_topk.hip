@@ -85,8 +85,9 @@ __global__ __launch_bounds__(64 * W, 4) void top_k_kernel(TopKArgs a)
   __shared__ CandidateBox<W> box;
   __shared__ double sums[W];
   maxima_ignore_nan();
-  const int r  = blockIdx.x;
-  const T* row = static_cast<const T*>(a.in) + (int64_t)r * a.ld;
+  const int64_t r = block_of_grid();
+  if (r >= a.n_rows) return;
+  const T* row = static_cast<const T*>(a.in) + r * a.ld;
   const int n  = a.n_cols;
   Running run;
   const Found f = stream_candidates<T, W, NV, Look::kEvery, SUM>(row, n, a.k, nullptr, a.scale, box, run);
@@ -105,7 +106,7 @@ __global__ __launch_bounds__(64 * W, 4) void top_k_kernel(TopKArgs a)
   auto write = [&](int j, u64 e) {
     const u32 key     = entry_key(e);
     const u32 i       = entry_index(e);
-    const int64_t out = (int64_t)r * a.k + j;
+    const int64_t out = r * a.k + j;
     // the key says the value but for the sign of a zero and the bits of a NaN
     if (key == 0 || key == 0x80000000u)
       static_cast<T*>(a.values)[out] = row[i];
@@ -134,7 +135,7 @@ __global__ __launch_bounds__(64 * W, 4) void top_k_kernel(TopKArgs a)
 template <class T, int W, int NV>
 int launch_rows(const TopKArgs& a, hipStream_t st)
 {
-  const dim3 grid((unsigned)a.n_rows), block(64 * W);
+  const dim3 grid = grid_of(a.n_rows), block(64 * W);
   if (a.lse != nullptr)
     hipLaunchKernelGGL((top_k_kernel<T, W, NV, true>), grid, block, 0, st, a);
   else

@@ -470,6 +470,31 @@ def test_sample_without_a_vocabulary(gpu):
     assert (token == -1).all() and (logprob == -INF).all()
 
 
+@pytest.mark.parametrize("rows", [(1 << 20) + 1, (1 << 24) + 3])
+def test_more_rows_than_one_grid_dimension_holds(gpu, rows):
+    """2^20 workgroups are one line of the grid; 2^24 of 256 threads would be 2^32 threads."""
+    import torch
+
+    from raft_amd import device
+    n = 3
+    x = torch.randn(rows, n, device="cuda", generator=torch.Generator("cuda").manual_seed(1)).half()
+    best = x.float().max(1)
+    values, indices = torch.empty(rows, 1, dtype=torch.float16, device="cuda"), torch.full((rows, 1), -1, dtype=torch.int32, device="cuda")
+    device.top_k(x, values, indices)
+    assert (values[:, 0].float() == best.values).all()
+    token = torch.full((rows,), -1, dtype=torch.int32, device="cuda")
+    zero = torch.zeros(rows, device="cuda")
+    device.sample(x, zero, token, temperature=zero)
+    assert (x.gather(1, token.long()[:, None])[:, 0].float() == best.values).all()
+    loss, stats, grad = torch.full((rows,), -1.0, device="cuda"), torch.empty(rows, 2, device="cuda"), torch.empty_like(x)
+    device.distill_loss(x, values, indices, loss, stats)
+    # one listed token has p = 1, so the loss is -log q
+    want = -torch.log_softmax(x.float(), 1).gather(1, indices.long())[:, 0]
+    assert (loss - want).abs().max() < 1e-5
+    device.distill_grad(x, values, indices, stats, grad)
+    assert grad.float().sum(1).abs().max() < 3 * 2.0 ** -11  # q - p sums to 0; three roundings
+
+
 # ---- together ---------------------------------------------------------------------------------------
 
 
