@@ -507,7 +507,7 @@ struct Found {
 // exponentials for the log-sum-exp, from the same loads.
 template <class T, int W, int NV, Look LOOK, bool SUM>
 __device__ __forceinline__ Found stream_candidates(const T* row, int n, int k, const u32* allowed, float c,
-                                                   CandidateBox<W>& box, Running& run)
+                                                   CandidateBox<W>& box, Running& run, bool sum = true)
 {
   constexpr int THREADS = 64 * W;
   constexpr int VEC     = In<T>::VEC;
@@ -527,7 +527,7 @@ __device__ __forceinline__ Found stream_candidates(const T* row, int n, int k, c
     if (LOOK != Look::kEvery && !(ext > -kInf)) ext_on = false;
   }
   if (!ext_on) ext = -kInf;
-  if (SUM && ext_on) {
+  if (SUM && sum && ext_on) {
     const float one[1][1] = {{ext}};
     run.raise(ext, c);
     run.add(one, c);
@@ -543,8 +543,9 @@ __device__ __forceinline__ Found stream_candidates(const T* row, int n, int k, c
     const u32 room = (u32)(left < BATCH ? left : BATCH) * 16u;
     u32 off        = (u32)(i * THREADS + tid) * 16u;
     off            = off < room ? off : room;
-    return __builtin_nontemporal_load(
-      reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(body + (int64_t)first * VEC) + off));
+    const char* p  = reinterpret_cast<const char*>(body + (int64_t)first * VEC) + off;
+    if constexpr (LOOK == Look::kEvery) return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+    else return *reinterpret_cast<const u32x4*>(p);  // sampling may come back to the row
   };
   // The elements of a vector; what does not count is -inf.
   auto unpack = [&](const u32x4& w, int v, float(&x)[VEC]) {
@@ -595,7 +596,7 @@ __device__ __forceinline__ Found stream_candidates(const T* row, int n, int k, c
       for (int p = 0; p < PAIR; ++p) m[i + p] = max_of(x[p]);
       const float most = max3(m[i], m[i + 1], -kInf);
       seen_max         = max3(seen_max, most, most);
-      if constexpr (SUM) {
+      if (SUM && sum) {
         run.raise(most, c);
         run.add(x, c);
       }

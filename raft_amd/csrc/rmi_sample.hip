@@ -23,161 +23,577 @@ struct SampleArgs {
 
 // exp((x - m) / T) as a whole number of 2^-bits: sums of such weights do not depend on how a row
 // is split or in which order it is added up, and they are exact.  n_cols * 2^bits stays below 2^63.
+//
+// With t = (x - m) log2(e) / T in 64 bits: t = k / 256 + f, 2^t = 2^(k >> 8) * table[k & 255] * 2^f,
+// |f| <= 1/512, and 2^f = 1 + f l + (f l)^2 / 2 + (f l)^3 / 6 with l = ln 2, off by (f l)^4 / 24 < 2^-42 / 24.
+// The last product adds 2^52, so the rounded weight stands in the low bits of the result.
+constexpr int kTable = 256;
 struct Weights {
-  double m, c, one;
-  float top;
+  const double* table;  // 2^(i / 256), in LDS
+  double m, c;          // t = (x - m) c
+  int bits;
+  bool infinite;        // the maximum is +inf: whatever else there is weighs nothing
+  // the weight + the bits of 2^52; not where the maximum is infinite
+  __device__ __forceinline__ u64 raw(float x) const
+  {
+    constexpr double kRound = 6755399441055744.0 / 256.0;  // 1.5 * 2^52 / 256: what is added to it is rounded to 1 / 256
+    constexpr double kL = kLn2, kL2 = kLn2 * kLn2 / 2, kL3 = kLn2 * kLn2 * kLn2 / 6;
+    // -inf, NaN and what is too small for a weight end at -64
+    const double t  = fmax(((double)x - m) * c, -64.0);
+    const double up = t + kRound;
+    const double f  = t - (up - kRound);
+    const int k     = (int)(u32)__builtin_bit_cast(u64, up);
+    const double p  = fma(fma(fma(kL3, f, kL2), f, kL), f, 1.0);
+    u64 scaled      = __builtin_bit_cast(u64, table[k & (kTable - 1)]);
+    scaled += (u64)(u32)(((k >> 8) + bits) << 20) << 32;
+    return __builtin_bit_cast(u64, fma(__builtin_bit_cast(double, scaled), p, 4503599627370496.0));
+  }
   __device__ __forceinline__ u64 operator()(float x) const
   {
-    // 2^52 + w holds w in its low bits; x == m also where both are infinite
-    const double t = x == top ? 0.0 : ((double)x - m) * c;
-    const double w = t > -64.0 ? exp2(t) : 0.0;
-    return __builtin_bit_cast(u64, fma(w, one, 4503599627370496.0)) & 0xfffffffffffffull;
+    if (infinite) return x == kInf ? (u64)1 << bits : 0;
+    return raw(x) & 0xfffffffffffffull;
   }
 };
 
-// One workgroup per row: one sweep for the maximum, sweeps for the cut by count and by mass, one
-// for the total, and one in index order that ends at the token.
-template <class T, int THREADS>
-__global__ __launch_bounds__(THREADS) void sample_kernel(SampleArgs a)
-{
-  constexpr int W   = THREADS / 64;
-  constexpr int VEC = In<T>::VEC;
-  __shared__ u64 bins[kBins + 2];
-  __shared__ u64 box[W];
-  __shared__ u64 found[2];
-  const int64_t r    = block_of_grid();
-  if (r >= a.n_rows) return;
-  const T* row       = static_cast<const T*>(a.logits) + r * a.ld;
-  const int n        = a.n_cols;
-  const u32* allowed = a.allowed != nullptr ? a.allowed + r * a.ld_allowed : nullptr;
-  auto eligible      = [&](float x, int i) {
-    return x > -kInf && (allowed == nullptr || ((allowed[i >> 5] >> (i & 31)) & 1u) != 0);
+struct Settings {
+  float temperature, top_p, min_p, u;
+  int top_k;
+  bool greedy;
+  __device__ __forceinline__ Settings(const SampleArgs& a, int64_t r)
+  {
+    temperature = a.temperature != nullptr ? a.temperature[r] : 1.0f;
+    greedy      = !(temperature > 0.0f);
+    if (greedy) temperature = 1.0f;
+    top_k = greedy ? 1 : (a.top_k != nullptr ? a.top_k[r] : 0);
+    top_p = !greedy && a.top_p != nullptr ? a.top_p[r] : 1.0f;
+    if (!(top_p < 1.0f)) top_p = 1.0f;
+    min_p = !greedy && a.min_p != nullptr ? a.min_p[r] : 0.0f;
+    min_p = min_p > 0.0f ? (min_p < 1.0f ? min_p : 1.0f) : 0.0f;
+    u     = a.u[r];
+  }
+  // the mass that has to be passed: the first element whose cumulative mass exceeds it is taken
+  __device__ __forceinline__ u64 goal(u64 all) const
+  {
+    const double at = (double)u * (double)all;
+    return at > 0 ? (at < (double)all ? min((u64)at, all - 1) : all - 1) : 0;
+  }
+  // a prefix in rank order is kept as long as the mass before an element is below this
+  __device__ __forceinline__ u64 nucleus(u64 all) const
+  {
+    const u64 mass = (u64)ceil((double)top_p * (double)all);
+    return mass > 1 ? mass : 1;
+  }
+};
+
+// What a workgroup keeps in LDS.
+template <int W>
+struct SampleBox {
+  static constexpr int kBinsOfT  = 256 * W;   // of the distance from the maximum, in log2
+  static constexpr int kSegments = 64 * W;
+  CandidateBox<W> c;                          // its `hit` and `bins` are free after the first pass
+  u64 sorted[kSegments];                      // candidates in rank order; later the sums of the segments
+  u64 mass[kSegments];
+  double table[kTable];
+  u64 box[W + 2];
+  float fbox[W];
+  u64 found[2];
+  u64 last;
+  int ibox[W];
+  int window[3];
+};
+
+// One row of a workgroup of W waves.
+template <class T, int W, bool MASKED>
+struct Row {
+  static constexpr int THREADS = 64 * W;
+  static constexpr int VEC     = In<T>::VEC;
+  const SampleArgs& a;
+  const T* row;
+  const u32* allowed;
+  SampleBox<W>& box;
+  const Settings& set;
+  Weights weight;
+  int n;
+  float max;
+  u64 least;  // that a weight has to be, for min_p
+  int64_t r;
+
+  __device__ __forceinline__ bool eligible(float x, int i) const
+  {
+    return x > -kInf && (!MASKED || ((allowed[i >> 5] >> (i & 31)) & 1u) != 0);
+  }
+  __device__ __forceinline__ void answer(int token, u64 mass, u64 all) const
+  {
+    a.token[r] = token;
+    if (a.logprob != nullptr) a.logprob[r] = (float)log((double)mass / (double)all);
+  }
+
+  // The token among the first `count` of box.sorted with their weights in box.mass, whose sum is `all`: the one, in
+  // index order, whose cumulative mass passes the goal.
+  __device__ void choose(int count, u64 all) const
+  {
+    const u64 goal = set.goal(all);
+    const int tid  = (int)threadIdx.x;
+    if (count <= 256) {
+      if ((tid & ~63) >= count) return;
+      const u32 mine = tid < count ? entry_index(box.sorted[tid]) : 0;
+      u64 upto       = 0;
+#pragma unroll 4
+      for (int o = 0; o < count; ++o) {
+        const u32 other = entry_index(box.sorted[o]);
+        upto += other <= mine ? box.mass[o] : 0;
+      }
+      if (tid < count && upto > goal && upto - box.mass[tid] <= goal) answer((int)mine, box.mass[tid], all);
+      return;
+    }
+    // the least index at which the mass up to it passes the goal, by halving
+    const u32 mine = tid < count ? entry_index(box.sorted[tid]) : ~0u;
+    const u64 own  = tid < count ? box.mass[tid] : 0;
+    u32 lo = 0, hi = (u32)n - 1;
+    while (lo < hi) {
+      const u32 mid  = lo + (hi - lo) / 2;
+      const u64 upto = block_all<W>(mine <= mid ? own : (u64)0, AddF{}, box.box);
+      if (upto > goal) hi = mid;
+      else lo = mid + 1;
+    }
+    if (mine == lo) answer((int)mine, own, all);
+  }
+
+  // Candidates into rank order, by counting for each those that rank before it; count <= THREADS.
+  __device__ void order(int count) const
+  {
+    const int tid = (int)threadIdx.x;
+    if ((tid & ~63) < count) {
+      const u64 own = tid < count ? box.c.entries[tid] : ~(u64)0;
+      int rank      = 0;
+#pragma unroll 4
+      for (int i = 0; i < count; ++i) rank += box.c.entries[i] > own;
+      if (tid < count) box.sorted[rank] = own;
+    }
+    __syncthreads();
+  }
+
+  // From the candidates alone, if they are sure to hold all that is kept; false if they are not.  `sum`,
+  // if there is a nucleus of the whole row, is the row's mass in fp32, right to within `off` of itself.
+  __device__ bool from_candidates(const Found& f, double sum, double off) const
+  {
+    const int tid = (int)threadIdx.x;
+    int count     = f.count;
+    if (!f.all) return false;
+    if (set.greedy) {  // the largest entry
+      u64 best = 0;
+      for (int i = tid; i < count; i += THREADS) best = best > box.c.entries[i] ? best : box.c.entries[i];
+      best = block_all<W>(best, [](u64 x, u64 y) { return x > y ? x : y; }, box.box);
+      if (tid == 0) answer((int)entry_index(best), 1, 1);
+      return true;
+    }
+    const bool by_k = set.top_k > 0;
+    if (count > THREADS) {
+      if (!by_k) return false;
+      thin_out<W>(box.c, count, set.top_k, f.tau, key32(f.max));
+      count = box.c.count;
+      if (count > THREADS) return false;
+    }
+    order(count);
+    const int kept = by_k && set.top_k < count ? set.top_k : count;
+    const u64 own  = tid < kept ? weight(value_of<float>(entry_key(box.sorted[tid]))) : 0;
+    u64 all;
+    const u64 before = block_before<W>(own, box.box, all);
+    if (tid < kept) box.mass[tid] = own;
+    // how many of the sorted candidates stay: at least `lo`, at most `hi`
+    int lo = kept, hi = kept;
+    bool open = !by_k && f.tau != 0;  // elements that are no candidates may belong to it
+    if (set.top_p < 1.0f) {
+      if (!open) {  // they are all there is
+        const u64 goal = set.nucleus(all);
+        lo = hi = block_all<W>(tid < kept && before < goal ? 1 : 0, AddF{}, box.ibox);
+      } else {
+        if (!(sum < 1e300) || !(off < 0.01)) return false;
+        const double goal = (double)set.top_p * sum;
+        lo = block_all<W>(tid < kept && (double)before < goal * (1 - off) ? 1 : 0, AddF{}, box.ibox);
+        hi = block_all<W>(tid < kept && (double)before < goal * (1 + off) + 1 ? 1 : 0, AddF{}, box.ibox);
+        // complete if the candidates' own mass passes the goal
+        open = !((double)all >= goal * (1 + off) + 1);
+      }
+    }
+    if (set.min_p > 0.0f) {
+      const int heavy = block_all<W>(tid < kept && own >= least ? 1 : 0, AddF{}, box.ibox);
+      lo = lo < heavy ? lo : heavy;
+      hi = hi < heavy ? hi : heavy;
+      if (heavy < kept) open = false;  // what ranks behind the candidates weighs less still
+    }
+    lo = lo > 1 ? lo : 1;  // the first stays whatever top_p is
+    if (lo != hi || open) return false;
+    if (tid == lo - 1) box.last = before + own;
+    __syncthreads();
+    choose(lo, box.last);
+    return true;
+  }
+
+  // The distance of an element from the maximum in parts of 48 / kBinsOfT powers of two.
+  struct Bin {
+    float c, r;
+    // 0 for the maximum, and larger behind it
+    __device__ __forceinline__ float place(float x) const
+    {
+      return fminf(fmaxf(fmaf(x, -c, r), 0.0f), (float)(SampleBox<W>::kBinsOfT - 1));
+    }
+    __device__ __forceinline__ int operator()(float x) const { return (int)place(x); }
   };
 
-  const float temperature = a.temperature != nullptr ? a.temperature[r] : 1.0f;
-  const bool greedy       = !(temperature > 0.0f);
-  float m                 = -kInf;
-  u64 count               = 0;
-  sweep<T, THREADS>(row, n, [&](float x, int i) {
-    if (eligible(x, i)) {
-      m = fmaxf(m, x);
-      ++count;
+  // A vector of a segment: its elements, -inf where there is none or it does not count.
+  __device__ __forceinline__ void elements(int at, float (&x)[VEC]) const
+  {
+    if (at + VEC <= n) {
+      const u32x4 w = load16c(row + at);
+      static_for<VEC>([&](auto j) { x[j] = (float)In<T>::template get<j>(w); });
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) x[j] = at + j < n ? widen(row + at + j) : -kInf;
     }
-  });
-  m     = block_all<W>(m, MaxF{}, reinterpret_cast<float*>(box));
-  count = block_all<W>(count, AddF{}, box);
-  if (count == 0) {
-    if (threadIdx.x == 0) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      if (MASKED) x[j] = at + j < n && eligible(x[j], at + j) ? x[j] : -kInf;
+      else x[j] = x[j] > -kInf ? x[j] : -kInf;  // NaN
+    }
+  }
+
+  static constexpr int kVectors = 4;                       // of a lane and segment
+  static constexpr int kSegment = 64 * VEC * kVectors;     // elements that one wave adds up
+
+  // Without top_k, where what is kept is more than the candidates: one exact pass that adds up every
+  // segment's weights.  For a nucleus a pass before it counts the elements by their distance from the
+  // maximum; the counts say between which distances the nucleus has to end, and the few elements there are
+  // put in order.  false if there are too many of them.
+  __device__ bool from_segments(double sum, double off) const
+  {
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int segments = (n + kSegment - 1) / kSegment;
+    if (segments > SampleBox<W>::kSegments || weight.infinite) return false;
+    constexpr int BINS = SampleBox<W>::kBinsOfT;
+    const float per    = (float)BINS / 48.0f;
+    const Bin bin{(float)weight.c * per, (float)(weight.m * weight.c) * per};
+    const bool nucleus = set.top_p < 1.0f;
+    int b0 = BINS, b1 = BINS;  // bins before b0 are kept whole, b1 and later ones not at all
+    if (nucleus) {
+      if (!(sum < 1e300) || !(off < 0.01)) return false;
+      // of every bin the number of elements (from bit 32 on) and the sum of their places in it (2^-12 of a bin)
+      u64* counts = reinterpret_cast<u64*>(box.c.hit);
+      static_assert(sizeof(box.c.hit) >= BINS * sizeof(u64), "the bins lie where the vectors were put aside");
+      __syncthreads();
+      for (int i = tid; i < BINS; i += THREADS) counts[i] = 0;
+      __syncthreads();
+      for (int s = wave; s < segments; s += W) {
+#pragma unroll
+        for (int v = 0; v < kVectors; ++v) {
+          float x[VEC];
+          elements(s * kSegment + (v * 64 + lane) * VEC, x);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            const float at = bin.place(x[j]);
+            const int b    = (int)at;
+            if (x[j] > -kInf)
+              atomicAdd((unsigned long long*)&counts[b], (1ull << 32) | (unsigned long long)(u32)((at - (float)b) * 4096.0f));
+          }
+        }
+      }
+      __syncthreads();
+      // every thread has a few bins; the mass up to and with a bin, right to some 1e-5 of itself
+      constexpr int EACH = BINS / THREADS;
+      const double one   = (double)((u64)1 << weight.bits);
+      auto mass_of       = [&](int b) {
+        const u64 w = counts[b];
+        const double count = (double)(u32)(w >> 32);
+        if (count == 0) return 0.0;
+        const double where = (double)b + (double)(u32)w / (4096.0 * count);
+        return count * one * exp2(-where * (48.0 / BINS));
+      };
+      double own = 0;
+      for (int e = 0; e < EACH; ++e) own += mass_of(tid * EACH + e);
+      double ignored;
+      double upto       = block_before<W>(own, reinterpret_cast<double*>(box.box), ignored);
+      const double goal = (double)set.top_p * sum;
+      const double give = off + 4e-5;
+      if (tid == 0) box.window[0] = box.window[1] = BINS;
+      __syncthreads();
+      for (int e = 0; e < EACH; ++e) {
+        const int b = tid * EACH + e;
+        upto += mass_of(b);
+        // the first bin that may hold the end, and the first that should lie behind it; the exact pass
+        // finds out whether that is so
+        if (upto >= goal * (1 - give)) atomicMin(&box.window[0], b);
+        if (upto >= goal * (1 + give) + 1) atomicMin(&box.window[1], b + 1);
+      }
+      __syncthreads();
+      b0 = box.window[0];
+      b1 = box.window[1];
+      u32 in = 0;
+      for (int e = 0; e < EACH; ++e) {
+        const int b = tid * EACH + e;
+        if (b >= b0 && b < b1) in += (u32)(counts[b] >> 32);
+      }
+      in = block_all<W>(in, AddF{}, reinterpret_cast<u32*>(box.ibox));
+      if (in > (u32)THREADS) return false;
+      if (tid == 0) box.c.count = 0;
+    }
+    __syncthreads();
+
+    // the exact pass.  raw() leaves 2^52's own bits in every weight; what was added of them is known.
+    constexpr u64 kHead = 0x4330000000000000ull;
+    u64 all             = 0;
+    for (int s = wave; s < segments; s += W) {
+      u64 sum_s = 0, sum_all = 0;
+#pragma unroll 1
+      for (int v = 0; v < kVectors; ++v) {
+        float x[VEC];
+        const int at = s * kSegment + (v * 64 + lane) * VEC;
+        elements(at, x);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const u64 w = weight.raw(x[j]) - kHead;
+          if (nucleus) {
+            sum_all += w;
+            const int b = bin(x[j]);
+            sum_s += b < b0 ? w : 0;
+            if (b >= b0 && b < b1 && x[j] > -kInf)
+              box.c.entries[atomicAdd(&box.c.count, 1)] = entry_of(key32(x[j]), (u32)(at + j));
+          } else {
+            sum_s += w >= least ? w : 0;
+          }
+        }
+      }
+      all += sum_all;
+      sum_s = wave_all(sum_s, AddF{});
+      if (lane == 0) box.mass[s] = sum_s;
+    }
+    __syncthreads();
+    u64 total = block_all<W>(tid < segments ? box.mass[tid] : (u64)0, AddF{}, box.box);
+    u64 last  = 0;  // the last entry kept of those between b0 and b1
+    if (nucleus) {
+      all            = block_all<W>(all, AddF{}, box.box);
+      const u64 goal = set.nucleus(all);
+      const int in   = box.c.count;
+      order(in);
+      const u64 e   = tid < in ? box.sorted[tid] : 0;
+      const u64 own = tid < in ? weight(value_of<float>(entry_key(e))) : 0;
+      u64 inside;
+      const u64 before = total + block_before<W>(own, box.box, inside);
+      // the nucleus ends where the counts said, or they were too coarse
+      if (!(total < goal && total + inside >= goal)) return false;
+      const bool stays = tid < in && before < goal;
+      if (stays) {
+        atomicAdd((unsigned long long*)&box.mass[entry_index(e) / kSegment], (unsigned long long)own);
+        if (before + own >= goal) {  // one thread
+          box.last     = e;
+          box.found[0] = before + own;
+          box.found[1] = own;
+        }
+      }
+      __syncthreads();
+      last  = box.last;
+      total = box.found[0];
+      // min_p may cut deeper: that is left to the general way
+      if (set.min_p > 0.0f && box.found[1] < least) return false;
+    }
+    // the segment, and in it the element, at which the mass passes the goal
+    const u64 goal = set.goal(total);
+    const u64 own  = tid < segments ? box.mass[tid] : 0;
+    u64 t2;
+    const u64 before = block_before<W>(own, box.box, t2);
+    __syncthreads();
+    if (before <= goal && before + own > goal) {
+      box.found[0]  = before;
+      box.window[0] = tid;
+    }
+    __syncthreads();
+    const int s   = box.window[0];
+    u64 upto      = box.found[0];
+    constexpr int EACH = (kSegment + THREADS - 1) / THREADS;
+    u64 w[EACH], mine = 0;
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      const int in = tid * EACH + e;
+      const int i  = s * kSegment + in;
+      w[e]         = 0;
+      if (in < kSegment && i < n) {
+        const float x = widen(row + i);
+        if (eligible(x, i)) {
+          w[e] = weight(x);
+          if (nucleus) {
+            const int b = bin(x);
+            if (b >= b1 || (b >= b0 && entry_of(key32(x), (u32)i) < last)) w[e] = 0;
+          } else if (w[e] < least) {
+            w[e] = 0;
+          }
+        }
+      }
+      mine += w[e];
+    }
+    upto += block_before<W>(mine, box.box, t2);
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      if (upto <= goal && upto + w[e] > goal) answer(s * kSegment + tid * EACH + e, w[e], total);
+      upto += w[e];
+    }
+    return true;
+  }
+
+  // Whatever the settings and the row are: sweeps for the cut by count and by mass (8 bits of the key
+  // each), one for the total, and one in index order that ends at the token.
+  __device__ void in_general(u64 count) const
+  {
+    u64* bins = box.c.entries;
+    // the cut in rank order: every element with a key above `key`, and with it up to index `last`
+    u32 key       = 0;
+    int last      = n;
+    u64 take      = ~(u64)0;  // elements with the key itself
+    u64 with      = 0;        // how many there are
+    const u32 top = key_of<T>(max);
+    if (set.top_k > 0 && (u64)set.top_k < count) {
+      const Cut c = find_cut<T, THREADS>(
+        row, n, top, (u64)set.top_k, [&](float x, int i) { return (u64)(eligible(x, i) ? 1 : 0); }, bins);
+      key  = c.key;
+      take = (u64)set.top_k - c.above;
+      with = c.with;
+    }
+    if (set.top_p < 1.0f) {
+      u64 all = 0;
+      sweep<T, THREADS>(row, n, [&](float x, int i) {
+        if (!eligible(x, i)) return;
+        const u32 k = key_of<T>(x);
+        if (k > key || (k == key && take == ~(u64)0)) all += weight(x);
+      });
+      all = block_all<W>(all, AddF{}, box.box);
+      if (take != ~(u64)0) all += take * weight(value_of<T>(key));
+      const u64 goal = set.nucleus(all);
+      if (goal < all) {
+        const Cut c = find_cut<T, THREADS>(
+          row, n, top, goal, [&](float x, int i) { return eligible(x, i) ? weight(x) : (u64)0; }, bins);
+        const u64 each = weight(value_of<T>(c.key));
+        key            = c.key;
+        take           = (goal - c.above + each - 1) / each;
+        with           = c.with / each;
+      }
+    }
+    if (take < with) {  // where the last of the equal elements is that is kept
+      u64 seen = 0;
+      ordered_sweep<T, THREADS>(row, n, [&](int at, const float(&x)[VEC], int cnt) {
+        u64 ties = 0;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          if (j < cnt && key_of<T>(x[j]) == key && eligible(x[j], at + j)) ++ties;
+        u64 all;
+        u64 rank = seen + block_before<W>(ties, box.box, all);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          if (j < cnt && key_of<T>(x[j]) == key && eligible(x[j], at + j) && ++rank == take) box.found[0] = (u64)(at + j);
+        seen += all;
+        return seen < take;
+      });
+      __syncthreads();
+      last = (int)box.found[0];
+    }
+    auto kept = [&](float x, int i) -> u64 {
+      if (!eligible(x, i)) return 0;
+      const u32 k = key_of<T>(x);
+      if (k < key || (k == key && i > last)) return 0;
+      const u64 w = weight(x);
+      return w >= least ? w : 0;
+    };
+    u64 all = 0;
+    sweep<T, THREADS>(row, n, [&](float x, int i) { all += kept(x, i); });
+    all            = block_all<W>(all, AddF{}, box.box);
+    const u64 goal = set.goal(all);
+    u64 seen       = 0;
+    ordered_sweep<T, THREADS>(row, n, [&](int at, const float(&x)[VEC], int cnt) {
+      u64 own[VEC], sum = 0;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) sum += own[j] = j < cnt ? kept(x[j], at + j) : 0;
+      u64 tile;
+      u64 upto = seen + block_before<W>(sum, box.box, tile);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        if (upto <= goal && upto + own[j] > goal) answer(at + j, own[j], all);
+        upto += own[j];
+      }
+      seen += tile;
+      return seen <= goal;
+    });
+  }
+};
+
+// One workgroup per row.  One pass finds the maximum, the elements that rank first and, where a nucleus is
+// asked for, the mass in fp32; that is enough wherever what is kept lies among some hundred elements.
+template <class T, int W, int NV, bool MASKED>
+__global__ __launch_bounds__(64 * W, 4) void sample_kernel(SampleArgs a)
+{
+  constexpr int THREADS = 64 * W;
+  __shared__ SampleBox<W> box;
+  maxima_ignore_nan();
+  const int64_t r = block_of_grid();
+  if (r >= a.n_rows) return;
+  const int tid = (int)threadIdx.x;
+  const int n   = a.n_cols;
+  const T* row  = static_cast<const T*>(a.logits) + r * a.ld;
+  const u32* allowed = MASKED ? a.allowed + r * a.ld_allowed : nullptr;
+  const Settings set(a, r);
+  for (int i = tid; i < kTable; i += THREADS) box.table[i] = exp2((double)i / kTable);
+
+  const bool sharp  = set.top_k > 0 && set.top_k <= 64 * W;
+  const bool some   = set.top_p < 1.0f || set.min_p > 0.0f;
+  const bool sum    = !sharp && set.top_p < 1.0f;
+  const int target  = sharp ? set.top_k : (some && set.top_k <= 0 ? 16 * W : 1);
+  const float c     = (float)(kLog2e / (double)set.temperature);
+  Running run;
+  const Found f = stream_candidates<T, W, NV, MASKED ? Look::kMasked : Look::kReal, true>(row, n, target, allowed, c, box.c,
+                                                                                           run, sum);
+  if (!(f.max > -kInf)) {  // nothing to choose from
+    if (tid == 0) {
       a.token[r] = -1;
       if (a.logprob != nullptr) a.logprob[r] = -kInf;
     }
     return;
   }
-  const u32 top = key_of<T>(m);
   Weights weight;
-  weight.m   = (double)m;
-  weight.top = m;
-  weight.c   = kLog2e / (greedy ? 1.0 : (double)temperature);
-  weight.one = (double)((u64)1 << a.bits);
-
-  // the cut in rank order: every element with a key above `key`, and with it up to index `last`
-  u32 key  = 0;
-  int last = n;
-  u64 take = ~(u64)0;  // elements with the key itself
-  const int want = greedy ? 1 : (a.top_k != nullptr ? a.top_k[r] : 0);
-  u64 with       = 0;  // how many there are
-  if (want > 0 && (u64)want < count) {
-    const Cut c = find_cut<T, THREADS>(
-      row, n, top, (u64)want, [&](float x, int i) { return (u64)(eligible(x, i) ? 1 : 0); }, bins);
-    key  = c.key;
-    take = (u64)want - c.above;
-    with = c.with;
+  weight.table    = box.table;
+  weight.m        = (double)f.max;
+  weight.c        = kLog2e / (double)set.temperature;
+  weight.bits     = a.bits;
+  weight.infinite = f.max == kInf;
+  const double one = (double)((u64)1 << a.bits);
+  const Row<T, W, MASKED> it{a, row, allowed, box, set, weight, n, f.max, (u64)ceil((double)set.min_p * one), r};
+  // The mass in fp32, and how far it may be off: n / THREADS additions in order and some 64 roundings of a term,
+  // as for a log-sum-exp, and the rounding of the reference that the terms are taken against; doubled.
+  double mass = 0, off = 0;
+  if (sum) {
+    mass = block_all<W>(run.against(f.max, c), AddF{}, reinterpret_cast<double*>(box.box)) * one;
+    off  = ((double)n / THREADS + 256.0 + fabs(weight.m * weight.c)) * 0x1p-23;
   }
-  const float top_p = !greedy && a.top_p != nullptr ? a.top_p[r] : 1.0f;
-  if (top_p < 1.0f) {
-    u64 all = 0;
-    sweep<T, THREADS>(row, n, [&](float x, int i) {
-      if (!eligible(x, i)) return;
-      const u32 k = key_of<T>(x);
-      if (k > key || (k == key && take == ~(u64)0)) all += weight(x);
-    });
-    all = block_all<W>(all, AddF{}, box);
-    if (take != ~(u64)0) all += take * weight(value_of<T>(key));
-    // an element is kept if the mass before it is below top_p of all
-    u64 goal = (u64)ceil((double)top_p * (double)all);
-    goal     = goal < 1 ? 1 : goal;
-    if (goal < all) {
-      const Cut c = find_cut<T, THREADS>(
-        row, n, top, goal, [&](float x, int i) { return eligible(x, i) ? weight(x) : (u64)0; }, bins);
-      const u64 each = weight(value_of<T>(c.key));
-      key            = c.key;
-      take           = (goal - c.above + each - 1) / each;
-      with           = c.with / each;
-    }
-  }
-  if (take < with) {  // where the last of the equal elements is that is kept
-    u64 seen = 0;
-    ordered_sweep<T, THREADS>(row, n, [&](int at, const float(&x)[VEC], int cnt) {
-      u64 ties = 0;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j)
-        if (j < cnt && key_of<T>(x[j]) == key && eligible(x[j], at + j)) ++ties;
-      u64 all;
-      u64 rank = seen + block_before<W>(ties, box, all);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j)
-        if (j < cnt && key_of<T>(x[j]) == key && eligible(x[j], at + j) && ++rank == take) found[0] = (u64)(at + j);
-      seen += all;
-      return seen < take;
-    });
-    __syncthreads();
-    last = (int)found[0];
-  }
-  const float min_p = !greedy && a.min_p != nullptr ? a.min_p[r] : 0.0f;
-  const double least = min_p > 0.0f ? fmin((double)min_p, 1.0) * weight.one : 0.0;
-  auto kept = [&](float x, int i) -> u64 {
-    if (!eligible(x, i)) return 0;
-    const u32 k = key_of<T>(x);
-    if (k < key || (k == key && i > last)) return 0;
-    const u64 w = weight(x);
-    return (double)w >= least ? w : 0;
-  };
-  u64 all = 0;
-  sweep<T, THREADS>(row, n, [&](float x, int i) { all += kept(x, i); });
-  all = block_all<W>(all, AddF{}, box);
-  // the first element, in index order, whose cumulative mass exceeds u * all
-  const double at_u = (double)a.u[r] * (double)all;
-  u64 goal          = at_u > 0 ? (at_u < (double)all ? (u64)at_u : all - 1) : 0;
-  goal              = goal < all ? goal : all - 1;
-  u64 seen          = 0;
-  ordered_sweep<T, THREADS>(row, n, [&](int at, const float(&x)[VEC], int cnt) {
-    u64 own[VEC], sum = 0;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) sum += own[j] = j < cnt ? kept(x[j], at + j) : 0;
-    u64 tile;
-    u64 upto = seen + block_before<W>(sum, box, tile);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      if (upto <= goal && upto + own[j] > goal) {
-        found[0] = (u64)(at + j);
-        found[1] = own[j];
-      }
-      upto += own[j];
-    }
-    seen += tile;
-    return seen <= goal;
-  });
+  if (set.greedy || sharp || (some && set.top_k <= 0))
+    if (it.from_candidates(f, mass, off)) return;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    a.token[r] = (int32_t)found[0];
-    if (a.logprob != nullptr) a.logprob[r] = (float)log((double)found[1] / (double)all);
-  }
+  if (set.top_k <= 0 || set.top_k >= n)
+    if (it.from_segments(mass, off)) return;
+  // the general way starts from the number of elements that count
+  u64 count = 0;
+  sweep<T, THREADS>(row, n, [&](float x, int i) { count += it.eligible(x, i) ? 1 : 0; });
+  count = block_all<W>(count, AddF{}, box.box);
+  it.in_general(count);
 }
 
 template <class T>
 int launch(const SampleArgs& a, hipStream_t st)
 {
-  hipLaunchKernelGGL((sample_kernel<T, 1024>), grid_of(a.n_rows), dim3(1024), 0, st, a);
+  const dim3 grid = grid_of(a.n_rows);
+  const bool wide = (int64_t)a.n_cols / In<T>::VEC > 1024;
+  if (wide && a.allowed != nullptr)
+    hipLaunchKernelGGL((sample_kernel<T, 16, 4, true>), grid, dim3(1024), 0, st, a);
+  else if (wide)
+    hipLaunchKernelGGL((sample_kernel<T, 16, 4, false>), grid, dim3(1024), 0, st, a);
+  else if (a.allowed != nullptr)
+    hipLaunchKernelGGL((sample_kernel<T, 4, 4, true>), grid, dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((sample_kernel<T, 4, 4, false>), grid, dim3(256), 0, st, a);
   return hipGetLastError() == hipSuccess ? RMI_OK : RMI_ERR_LAUNCH;
 }
 
