@@ -101,8 +101,28 @@ __device__ __forceinline__ T wave_all(T v, F f)
   return v;
 }
 
-// f over all threads of a workgroup of W waves, in wave order (the same bits every time); `box`
-// holds W values and is free again after the next barrier.
+// f over the first W lanes' values, for all lanes (W a power of two, at most 16).
+template <int W, class T, class F>
+__device__ __forceinline__ T lanes_all(T v, F f)
+{
+  static_assert(W <= 16 && (W & (W - 1)) == 0, "within a row of 16 lanes");
+  if constexpr (W > 1) v = f(v, xchg<0>(v));
+  if constexpr (W > 2) v = f(v, xchg<1>(v));
+  if constexpr (W > 4) v = f(v, xchg<2>(v));
+  if constexpr (W > 8) v = f(v, xchg<3>(v));
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
+  } else {
+    const u64 w  = __builtin_bit_cast(u64, v);
+    const u32 lo = (u32)__builtin_amdgcn_readfirstlane((int)(u32)w);
+    const u32 hi = (u32)__builtin_amdgcn_readfirstlane((int)(u32)(w >> 32));
+    return __builtin_bit_cast(T, ((u64)hi << 32) | lo);
+  }
+}
+
+// f over all threads of a workgroup of W waves (the same bits every time); `box` holds W values and is
+// free again after the next barrier.  Lane w of every wave takes wave w's value: a few steps instead of
+// a walk over all of them, whose instructions count where a kernel runs its code once.
 template <int W, class T, class F>
 __device__ __forceinline__ T block_all(T v, F f, T* box)
 {
@@ -111,9 +131,7 @@ __device__ __forceinline__ T block_all(T v, F f, T* box)
     __syncthreads();
     if ((threadIdx.x & 63) == 0) box[threadIdx.x >> 6] = v;
     __syncthreads();
-    v = box[0];
-#pragma unroll
-    for (int w = 1; w < W; ++w) v = f(v, box[w]);
+    v = lanes_all<W>(box[threadIdx.x & (W - 1)], f);
   }
   return v;
 }
@@ -144,14 +162,10 @@ __device__ __forceinline__ T block_before(T v, T* box, T& total)
   __syncthreads();
   if (lane == 63) box[threadIdx.x >> 6] = s;
   __syncthreads();
-  T before = s - v;
-  total    = 0;
-#pragma unroll
-  for (int w = 0; w < W; ++w) {
-    if (w < (int)(threadIdx.x >> 6)) before += box[w];
-    total += box[w];
-  }
-  return before;
+  const T own     = box[lane & (W - 1)];
+  total           = lanes_all<W>(own, AddF{});
+  const T earlier = lanes_all<W>((lane & (W - 1)) < (int)(threadIdx.x >> 6) ? own : (T)0, AddF{});
+  return earlier + (s - v);
 }
 
 // ---- sweeps -------------------------------------------------------------------------------------
@@ -169,21 +183,40 @@ __device__ __forceinline__ void sweep(const T* row, int n, F f)
   for (int i = nv * VEC + threadIdx.x; i < n; i += THREADS) f(widen(row + i), i);
 }
 
-// Visits the row in index order, a tile of THREADS vectors at a time: g(first index, values,
+// The same element by element, four at a time: a fifth of the code and of the registers, for ways that are
+// rarely taken in a kernel that has others.
+template <class T, int THREADS, class F>
+__device__ __forceinline__ void narrow_sweep(const T* row, int n, F f)
+{
+  for (int first = threadIdx.x; first < n; first += 4 * THREADS) {
+    float x[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = first + u * THREADS;
+      x[u]        = widen(row + (i < n ? i : first));
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (first + u * THREADS < n) f(x[u], first + u * THREADS);
+  }
+}
+
+// Visits the row in index order, a tile of VEC elements a thread at a time: g(first index, values,
 // count) in every thread, count elements from that index on, until g returns false (in every
 // thread alike).  All threads call g for every tile.
-template <class T, int THREADS, class G>
+template <class T, int THREADS, int VEC = In<T>::VEC, class G>
 __device__ __forceinline__ void ordered_sweep(const T* row, int n, G g)
 {
-  constexpr int VEC = In<T>::VEC;
   for (int base = 0; base < n; base += THREADS * VEC) {
     const int at = base + (int)threadIdx.x * VEC;
     float x[VEC];
     int count = n - at;
     count     = count < 0 ? 0 : (count > VEC ? VEC : count);
-    if (count == VEC) {
-      const u32x4 w = load16c(row + at);
-      static_for<VEC>([&](auto j) { x[j] = (float)In<T>::template get<j>(w); });
+    if (VEC == In<T>::VEC && count == VEC) {
+      if constexpr (VEC == In<T>::VEC) {
+        const u32x4 w = load16c(row + at);
+        static_for<VEC>([&](auto j) { x[j] = (float)In<T>::template get<j>(w); });
+      }
     } else {
 #pragma unroll
       for (int j = 0; j < VEC; ++j) x[j] = j < count ? widen(row + at + j) : 0.0f;
@@ -208,8 +241,8 @@ constexpr int kBins = 256;
 // of keys that is left into 256 parts and adds the elements' weights up in LDS: one sweep for each
 // 8 bits of the range.  The weights are whole numbers, so the order of the additions does not
 // matter.  weigh(x, index) is 0 for elements that do not count.
-template <class T, int THREADS, class F>
-__device__ Cut find_cut(const T* row, int n, u32 max_key, u64 target, F weigh, u64* bins /* kBins + 2 */)
+template <class T, int THREADS, bool NARROW = false, class F>
+__device__ __forceinline__ Cut find_cut(const T* row, int n, u32 max_key, u64 target, F weigh, u64* bins /* kBins + 2 */)
 {
   u32 lo = 0, hi = max_key;
   u64 above = 0;
@@ -224,12 +257,16 @@ __device__ Cut find_cut(const T* row, int n, u32 max_key, u64 target, F weigh, u
       bins[kBins + 1] = 0;
     }
     __syncthreads();
-    sweep<T, THREADS>(row, n, [&](float x, int i) {
+    auto add = [&](float x, int i) {
       const u32 k = key_of<T>(x);
       if (k < lo || k > hi) return;
       const u64 w = weigh(x, i);
       if (w != 0) atomicAdd((unsigned long long*)&bins[(k - lo) >> shift], (unsigned long long)w);
-    });
+    };
+    if constexpr (NARROW)
+      narrow_sweep<T, THREADS>(row, n, add);
+    else
+      sweep<T, THREADS>(row, n, add);
     __syncthreads();
     if (threadIdx.x < 64) {  // the first wave: from the last bin down, four bins a lane
       const int l = 63 - (int)threadIdx.x;
@@ -358,7 +395,7 @@ __device__ __forceinline__ u32 key32(float x) { return key_of<float>(x); }
 // equal parts of the range between the least and the largest of them, and everything below the part
 // that holds the k-th is dropped.  Returns the lower edge of that part; box.count is the new count.
 template <int W>
-__device__ u32 thin_out(CandidateBox<W>& box, int count, int k, u32 lo, u32 hi)
+__device__ __forceinline__ u32 thin_out(CandidateBox<W>& box, int count, int k, u32 lo, u32 hi)
 {
   constexpr int THREADS = 64 * W;
   constexpr int EACH    = CandidateBox<W>::kEntries / THREADS;
@@ -488,6 +525,26 @@ struct Running {
     return (fabsf(top) < kLarge ? (double)(ref(top) * c) * kLn2 : (double)ref(top) * inv_t) + log(all);
   }
 };
+
+// Descending, `size` (a power of two) entries.
+template <int THREADS>
+__device__ __forceinline__ void sort_entries(u64* e, int size)
+{
+  for (int len = 2; len <= size; len <<= 1) {
+    for (int d = len >> 1; d > 0; d >>= 1) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < size / 2; i += THREADS) {
+        const int a = 2 * i - (i & (d - 1));
+        const u64 x = e[a], y = e[a + d];
+        if ((x < y) == ((a & len) == 0)) {
+          e[a]     = y;
+          e[a + d] = x;
+        }
+      }
+    }
+  }
+  __syncthreads();
+}
 
 struct Found {
   bool all;    // the box holds the candidates; otherwise they did not fit and it is of no use
@@ -656,6 +713,7 @@ __device__ __forceinline__ Found stream_candidates(const T* row, int n, int k, c
   auto gather = [&](bool more) {
     __syncthreads();
     const int hits = box.hits;
+    __syncthreads();  // every wave has read it before a fast one adds the next batch's
     if (hits > CandidateBox<W>::kHits) {  // what is left of the row is read for its maximum and sum
       fits     = false;
       at_least = __builtin_nanf("");

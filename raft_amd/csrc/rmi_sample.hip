@@ -3,6 +3,8 @@
 #include "rmi_logits.hpp"
 
 namespace rmi {
+int cu_count();  // rmi_api.hip
+
 namespace logits {
 namespace {
 
@@ -55,6 +57,10 @@ struct Weights {
   }
 };
 
+struct MaxI {
+  __device__ __forceinline__ int operator()(int a, int b) const { return a > b ? a : b; }
+};
+
 struct Settings {
   float temperature, top_p, min_p, u;
   int top_k;
@@ -88,9 +94,9 @@ struct Settings {
 // What a workgroup keeps in LDS.
 template <int W>
 struct SampleBox {
-  static constexpr int kBinsOfT  = 256 * W;   // of the distance from the maximum, in log2
+  static constexpr int kBinsOfT  = 1024 * W;  // of the distance from the maximum, in log2
   static constexpr int kSegments = 64 * W;
-  CandidateBox<W> c;                          // its `hit` and `bins` are free after the first pass
+  CandidateBox<W> c;                          // its entries and hits make room for the bins
   u64 sorted[kSegments];                      // candidates in rank order; later the sums of the segments
   u64 mass[kSegments];
   double table[kTable];
@@ -130,7 +136,7 @@ struct Row {
 
   // The token among the first `count` of box.sorted with their weights in box.mass, whose sum is `all`: the one, in
   // index order, whose cumulative mass passes the goal.
-  __device__ void choose(int count, u64 all) const
+  __device__ __forceinline__ void choose(int count, u64 all) const
   {
     const u64 goal = set.goal(all);
     const int tid  = (int)threadIdx.x;
@@ -159,23 +165,54 @@ struct Row {
     if (mine == lo) answer((int)mine, own, all);
   }
 
-  // Candidates into rank order, by counting for each those that rank before it; count <= THREADS.
-  __device__ void order(int count) const
+  // Candidates into rank order (count <= THREADS): few by counting for each those that rank before it, more by
+  // sorting, which is a handful of steps to LDS against one for every candidate.
+  __device__ __forceinline__ void order(int count) const
   {
     const int tid = (int)threadIdx.x;
-    if ((tid & ~63) < count) {
-      const u64 own = tid < count ? box.c.entries[tid] : ~(u64)0;
-      int rank      = 0;
+    if (count <= 256) {
+      if ((tid & ~63) < count) {
+        const u64 own = tid < count ? box.c.entries[tid] : ~(u64)0;
+        int rank      = 0;
 #pragma unroll 4
-      for (int i = 0; i < count; ++i) rank += box.c.entries[i] > own;
-      if (tid < count) box.sorted[rank] = own;
+        for (int i = 0; i < count; ++i) rank += box.c.entries[i] > own;
+        if (tid < count) box.sorted[rank] = own;
+      }
+      __syncthreads();
+      return;
     }
+    int size = 512;
+    while (size < count) size <<= 1;
+    if (tid >= count && tid < size) box.c.entries[tid] = 0;
+    sort_entries<THREADS>(box.c.entries, size);
+    if (tid < count) box.sorted[tid] = box.c.entries[tid];
     __syncthreads();
   }
 
+  // The distance of an element from the maximum in parts of 48 / kBinsOfT powers of two.
+  struct Bin {
+    float c, r;
+    // 0 for the maximum, and larger behind it
+    __device__ __forceinline__ float place(float x) const
+    {
+      return fminf(fmaxf(fmaf(x, -c, r), 0.0f), (float)(SampleBox<W>::kBinsOfT - 1));
+    }
+    __device__ __forceinline__ int operator()(float x) const { return (int)place(x); }
+  };
+
+  __device__ __forceinline__ Bin bins() const
+  {
+    const float per = (float)SampleBox<W>::kBinsOfT / 48.0f;
+    return Bin{(float)weight.c * per, (float)(weight.m * weight.c) * per};
+  }
+
+  // How many candidates are looked for where their number is not given.
+  static constexpr int kNucleus = 12 * W;
+
   // From the candidates alone, if they are sure to hold all that is kept; false if they are not.  `sum`,
   // if there is a nucleus of the whole row, is the row's mass in fp32, right to within `off` of itself.
-  __device__ bool from_candidates(const Found& f, double sum, double off) const
+  // `base` and `known`: the exact mass of all values in the first `known` bins (see Bin).
+  __device__ __forceinline__ bool from_candidates(const Found& f, double sum, double off, u64& base, int& known) const
   {
     const int tid = (int)threadIdx.x;
     int count     = f.count;
@@ -188,9 +225,10 @@ struct Row {
       return true;
     }
     const bool by_k = set.top_k > 0;
-    if (count > THREADS) {
-      if (!by_k) return false;
-      thin_out<W>(box.c, count, set.top_k, f.tau, key32(f.max));
+    u32 tau        = f.tau;
+    const int target = by_k ? set.top_k : kNucleus;
+    if (count > target + target / 4 || count > THREADS) {  // fewer to put in order: one a thread at most
+      tau   = thin_out<W>(box.c, count, target, tau, key32(f.max));
       count = box.c.count;
       if (count > THREADS) return false;
     }
@@ -202,7 +240,7 @@ struct Row {
     if (tid < kept) box.mass[tid] = own;
     // how many of the sorted candidates stay: at least `lo`, at most `hi`
     int lo = kept, hi = kept;
-    bool open = !by_k && f.tau != 0;  // elements that are no candidates may belong to it
+    bool open = !by_k && tau != 0;  // elements that are no candidates may belong to it
     if (set.top_p < 1.0f) {
       if (!open) {  // they are all there is
         const u64 goal = set.nucleus(all);
@@ -214,6 +252,20 @@ struct Row {
         hi = block_all<W>(tid < kept && (double)before < goal * (1 + off) + 1 ? 1 : 0, AddF{}, box.ibox);
         // complete if the candidates' own mass passes the goal
         open = !((double)all >= goal * (1 + off) + 1);
+        // for the other way: the last bin that is well inside, and the mass up to its end
+        const Bin bin  = bins();
+        const int mine = tid < kept ? bin(value_of<float>(entry_key(box.sorted[tid]))) : 0;
+        const bool ends = tid + 1 < kept && mine != bin(value_of<float>(entry_key(box.sorted[tid + 1])));
+        const int inside = block_all<W>(ends && (double)(before + own) < goal * 0.997 ? tid + 1 : 0, MaxI{}, box.ibox);
+        if (inside > 0) {
+          if (tid == inside - 1) {
+            box.found[0] = before + own;
+            box.found[1] = (u64)mine + 1;
+          }
+          __syncthreads();
+          base  = box.found[0];
+          known = (int)box.found[1];
+        }
       }
     }
     if (set.min_p > 0.0f) {
@@ -230,142 +282,188 @@ struct Row {
     return true;
   }
 
-  // The distance of an element from the maximum in parts of 48 / kBinsOfT powers of two.
-  struct Bin {
-    float c, r;
-    // 0 for the maximum, and larger behind it
-    __device__ __forceinline__ float place(float x) const
-    {
-      return fminf(fmaxf(fmaf(x, -c, r), 0.0f), (float)(SampleBox<W>::kBinsOfT - 1));
-    }
-    __device__ __forceinline__ int operator()(float x) const { return (int)place(x); }
-  };
-
-  // A vector of a segment: its elements, -inf where there is none or it does not count.
-  __device__ __forceinline__ void elements(int at, float (&x)[VEC]) const
+  // The least value whose bin lies before b; NaN if there is none.  Bins fall as values rise.
+  __device__ __forceinline__ float least_in(const Bin& bin, int b) const
   {
-    if (at + VEC <= n) {
-      const u32x4 w = load16c(row + at);
-      static_for<VEC>([&](auto j) { x[j] = (float)In<T>::template get<j>(w); });
-    } else {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) x[j] = at + j < n ? widen(row + at + j) : -kInf;
+    u32 lo = key32(-3.402823466e38f), hi = key32(max);
+    if (bin(max) >= b) return __builtin_nanf("");
+    while (lo < hi) {
+      const u32 mid = lo + (hi - lo) / 2;
+      if (bin(value_of<float>(mid)) < b) hi = mid;
+      else lo = mid + 1;
     }
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      if (MASKED) x[j] = at + j < n && eligible(x[j], at + j) ? x[j] : -kInf;
-      else x[j] = x[j] > -kInf ? x[j] : -kInf;  // NaN
-    }
+    return value_of<float>(lo);
   }
 
-  static constexpr int kVectors = 4;                       // of a lane and segment
+  static constexpr int kVectors = 4;                   // of a lane and segment
   static constexpr int kSegment = 64 * VEC * kVectors;     // elements that one wave adds up
+
+  // A lane's vectors of one segment as they were loaded, with the mask's bits.
+  struct Loaded {
+    u32x4 w[kVectors];
+    u32 bits[kVectors];
+  };
+
+  // g(segment, index of the first element, VEC elements) for every vector of the row that this wave has: the
+  // waves take the segments in turn, and load the next one before they work on one.  What the mask
+  // leaves out, or lies behind the row's end, is -inf; NaN is left as it is.
+  template <class G>
+  __device__ __forceinline__ void segments_of_wave(G g) const
+  {
+    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+    const int whole = n / kSegment;
+    const int words = (n + 31) >> 5;
+    auto load = [&](int s) {
+      Loaded l;
+#pragma unroll
+      for (int v = 0; v < kVectors; ++v) {
+        const int at = s * kSegment + (v * 64 + lane) * VEC;
+        l.w[v]       = load16c(row + at);
+        l.bits[v]    = MASKED ? mask_bits(allowed, at, words) : 0;
+      }
+      return l;
+    };
+    auto unpack = [&](const u32x4& w, u32 bits, float(&x)[VEC]) {
+      static_for<VEC>([&](auto j) { x[j] = (float)In<T>::template get<j>(w); });
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        if (MASKED) x[j] = ((bits >> j) & 1u) != 0 ? x[j] : -kInf;
+    };
+    if (wave < whole) {
+      Loaded now = load(wave);
+      for (int s = wave; s < whole; s += W) {
+        const Loaded next = load(s + W < whole ? s + W : s);
+#pragma unroll
+        for (int v = 0; v < kVectors; ++v) {
+          float x[VEC];
+          unpack(now.w[v], now.bits[v], x);
+          g(s, s * kSegment + (v * 64 + lane) * VEC, x);
+        }
+        now = next;
+      }
+    }
+    if (whole * kSegment < n && wave == whole % W) {  // the last, partly filled segment
+#pragma unroll 1
+      for (int v = 0; v < kVectors; ++v) {
+        const int at = whole * kSegment + (v * 64 + lane) * VEC;
+        float x[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          x[j] = at + j < n ? widen(row + at + j) : -kInf;
+          x[j] = at + j < n && eligible(x[j], at + j) ? x[j] : -kInf;
+        }
+        g(whole, at, x);
+      }
+    }
+  }
 
   // Without top_k, where what is kept is more than the candidates: one exact pass that adds up every
   // segment's weights.  For a nucleus a pass before it counts the elements by their distance from the
   // maximum; the counts say between which distances the nucleus has to end, and the few elements there are
   // put in order.  false if there are too many of them.
-  __device__ bool from_segments(double sum, double off) const
+  __device__ __forceinline__ bool from_segments(double sum, double off, u64 base, int known) const
   {
-    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = (int)threadIdx.x, lane = tid & 63;
     const int segments = (n + kSegment - 1) / kSegment;
     if (segments > SampleBox<W>::kSegments || weight.infinite) return false;
     constexpr int BINS = SampleBox<W>::kBinsOfT;
-    const float per    = (float)BINS / 48.0f;
-    const Bin bin{(float)weight.c * per, (float)(weight.m * weight.c) * per};
+    const Bin bin      = bins();
     const bool nucleus = set.top_p < 1.0f;
-    int b0 = BINS, b1 = BINS;  // bins before b0 are kept whole, b1 and later ones not at all
+    // what is kept whole, and what may be kept: values from here on (NaN: none)
+    float above = -kInf, low = -kInf;
     if (nucleus) {
       if (!(sum < 1e300) || !(off < 0.01)) return false;
-      // of every bin the number of elements (from bit 32 on) and the sum of their places in it (2^-12 of a bin)
-      u64* counts = reinterpret_cast<u64*>(box.c.hit);
-      static_assert(sizeof(box.c.hit) >= BINS * sizeof(u64), "the bins lie where the vectors were put aside");
+      u32* counts = reinterpret_cast<u32*>(&box.c);
+      // (64 more for what does not count, one a lane, so that no two lanes meet there)
+      static_assert(offsetof(CandidateBox<W>, bins) >= (BINS + 64) * sizeof(u32), "the bins fit into what is free");
       __syncthreads();
       for (int i = tid; i < BINS; i += THREADS) counts[i] = 0;
       __syncthreads();
-      for (int s = wave; s < segments; s += W) {
+      segments_of_wave([&](int, int, const float(&x)[VEC]) {
 #pragma unroll
-        for (int v = 0; v < kVectors; ++v) {
-          float x[VEC];
-          elements(s * kSegment + (v * 64 + lane) * VEC, x);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const float at = bin.place(x[j]);
-            const int b    = (int)at;
-            if (x[j] > -kInf)
-              atomicAdd((unsigned long long*)&counts[b], (1ull << 32) | (unsigned long long)(u32)((at - (float)b) * 4096.0f));
-          }
-        }
-      }
+        for (int j = 0; j < VEC; ++j) atomicAdd(&counts[x[j] > -kInf ? bin(x[j]) : BINS + lane], 1u);
+      });
       __syncthreads();
-      // every thread has a few bins; the mass up to and with a bin, right to some 1e-5 of itself
+      // Every thread has a few bins; the mass up to and with a bin, as if its elements lay in its middle.  That
+      // would be far off for the few heaviest, whose mass is known.
       constexpr int EACH = BINS / THREADS;
       const double one   = (double)((u64)1 << weight.bits);
       auto mass_of       = [&](int b) {
-        const u64 w = counts[b];
-        const double count = (double)(u32)(w >> 32);
-        if (count == 0) return 0.0;
-        const double where = (double)b + (double)(u32)w / (4096.0 * count);
-        return count * one * exp2(-where * (48.0 / BINS));
+        const u32 count = b < known ? 0 : counts[b];
+        return count != 0 ? (double)count * one * (double)__builtin_amdgcn_exp2f(-((float)b + 0.5f) * (48.0f / BINS)) : 0.0;
       };
       double own = 0;
       for (int e = 0; e < EACH; ++e) own += mass_of(tid * EACH + e);
       double ignored;
-      double upto       = block_before<W>(own, reinterpret_cast<double*>(box.box), ignored);
+      double upto       = (double)base + block_before<W>(own, reinterpret_cast<double*>(box.box), ignored);
       const double goal = (double)set.top_p * sum;
-      const double give = off + 4e-5;
+      // bins are 0.2 or 0.4 % wide, and the places of many values in theirs average out
+      const double give = off + 2e-4;
       if (tid == 0) box.window[0] = box.window[1] = BINS;
       __syncthreads();
       for (int e = 0; e < EACH; ++e) {
-        const int b = tid * EACH + e;
+        const int b       = tid * EACH + e;
+        const double less = b == 0 ? -1.0 : upto;
         upto += mass_of(b);
-        // the first bin that may hold the end, and the first that should lie behind it; the exact pass
-        // finds out whether that is so
-        if (upto >= goal * (1 - give)) atomicMin(&box.window[0], b);
-        if (upto >= goal * (1 + give) + 1) atomicMin(&box.window[1], b + 1);
+        // the first bin that may hold the end, and the first that should lie behind it (one thread each); the
+        // exact pass finds out whether that is so
+        if (less < goal * (1 - give) && upto >= goal * (1 - give)) box.window[0] = b;
+        if (less < goal * (1 + give) + 1 && upto >= goal * (1 + give) + 1) box.window[1] = b + 1;
       }
       __syncthreads();
-      b0 = box.window[0];
-      b1 = box.window[1];
+      // bins before b0 are kept whole, b1 and later ones not at all
+      const int b0 = box.window[0] > known ? box.window[0] : known, b1 = box.window[1];
       u32 in = 0;
       for (int e = 0; e < EACH; ++e) {
         const int b = tid * EACH + e;
-        if (b >= b0 && b < b1) in += (u32)(counts[b] >> 32);
+        if (b >= b0 && b < b1) in += counts[b];
       }
       in = block_all<W>(in, AddF{}, reinterpret_cast<u32*>(box.ibox));
-      if (in > (u32)THREADS) return false;
+      if (in > (u32)CandidateBox<W>::kEntries) return false;
       if (tid == 0) box.c.count = 0;
+      above = least_in(bin, b0);
+      low   = least_in(bin, b1);
     }
     __syncthreads();
 
-    // the exact pass.  raw() leaves 2^52's own bits in every weight; what was added of them is known.
+    // the exact pass.  Every weight comes with the bits of 2^52; what was added of them is taken off at the end.
     constexpr u64 kHead = 0x4330000000000000ull;
-    u64 all             = 0;
-    for (int s = wave; s < segments; s += W) {
-      u64 sum_s = 0, sum_all = 0;
-#pragma unroll 1
-      for (int v = 0; v < kVectors; ++v) {
-        float x[VEC];
-        const int at = s * kSegment + (v * 64 + lane) * VEC;
-        elements(at, x);
+    u64 all = 0, sum_s = 0, added = 0;
+    int at_segment = -1;
+    auto close     = [&]() {  // this wave's segment is complete
+      if (at_segment < 0) return;
+      const u64 w = wave_all(sum_s, AddF{});
+      if (lane == 0) box.mass[at_segment] = w;
+      sum_s = 0;
+    };
+    segments_of_wave([&](int s, int at, const float(&x)[VEC]) {
+      if (s != at_segment) {
+        close();
+        at_segment = s;
+      }
+      u64 w[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) w[j] = weight.raw(x[j]);
+      u64 part = 0;
+      if (nucleus) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          const u64 w = weight.raw(x[j]) - kHead;
-          if (nucleus) {
-            sum_all += w;
-            const int b = bin(x[j]);
-            sum_s += b < b0 ? w : 0;
-            if (b >= b0 && b < b1 && x[j] > -kInf)
-              box.c.entries[atomicAdd(&box.c.count, 1)] = entry_of(key32(x[j]), (u32)(at + j));
-          } else {
-            sum_s += w >= least ? w : 0;
-          }
+          all += w[j];
+          const bool kept = x[j] >= above;
+          part += kept ? w[j] : kHead;
+          if (x[j] >= low && !kept)
+            box.c.entries[atomicAdd(&box.c.count, 1)] = entry_of(key32(x[j]), (u32)(at + j));
         }
+        added += VEC * kHead;
+      } else {
+        const u64 from = least + kHead;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) part += w[j] >= from ? w[j] : kHead;
       }
-      all += sum_all;
-      sum_s = wave_all(sum_s, AddF{});
-      if (lane == 0) box.mass[s] = sum_s;
-    }
+      sum_s += part - VEC * kHead;
+    });
+    close();
+    all -= added;
     __syncthreads();
     u64 total = block_all<W>(tid < segments ? box.mass[tid] : (u64)0, AddF{}, box.box);
     u64 last  = 0;  // the last entry kept of those between b0 and b1
@@ -373,21 +471,35 @@ struct Row {
       all            = block_all<W>(all, AddF{}, box.box);
       const u64 goal = set.nucleus(all);
       const int in   = box.c.count;
-      order(in);
-      const u64 e   = tid < in ? box.sorted[tid] : 0;
-      const u64 own = tid < in ? weight(value_of<float>(entry_key(e))) : 0;
+      u64* entries   = box.c.entries;
+      int size       = 2;
+      while (size < in) size <<= 1;
+      for (int i = in + tid; i < size; i += THREADS) entries[i] = 0;
+      sort_entries<THREADS>(entries, size);
+      constexpr int EACH = CandidateBox<W>::kEntries / THREADS;  // consecutive ones
+      u64 w[EACH], mine = 0;
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        const int i = tid * EACH + e;
+        w[e]        = i < in ? weight(value_of<float>(entry_key(entries[i]))) : 0;
+        mine += w[e];
+      }
       u64 inside;
-      const u64 before = total + block_before<W>(own, box.box, inside);
+      u64 before = total + block_before<W>(mine, box.box, inside);
       // the nucleus ends where the counts said, or they were too coarse
       if (!(total < goal && total + inside >= goal)) return false;
-      const bool stays = tid < in && before < goal;
-      if (stays) {
-        atomicAdd((unsigned long long*)&box.mass[entry_index(e) / kSegment], (unsigned long long)own);
-        if (before + own >= goal) {  // one thread
-          box.last     = e;
-          box.found[0] = before + own;
-          box.found[1] = own;
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        const int i = tid * EACH + e;
+        if (i < in && before < goal) {
+          atomicAdd((unsigned long long*)&box.mass[entry_index(entries[i]) / kSegment], (unsigned long long)w[e]);
+          if (before + w[e] >= goal) {  // one thread
+            box.last     = entries[i];
+            box.found[0] = before + w[e];
+            box.found[1] = w[e];
+          }
         }
+        before += w[e];
       }
       __syncthreads();
       last  = box.last;
@@ -420,8 +532,7 @@ struct Row {
         if (eligible(x, i)) {
           w[e] = weight(x);
           if (nucleus) {
-            const int b = bin(x);
-            if (b >= b1 || (b >= b0 && entry_of(key32(x), (u32)i) < last)) w[e] = 0;
+            if (!(x >= above) && !(x >= low && entry_of(key32(x), (u32)i) >= last)) w[e] = 0;
           } else if (w[e] < least) {
             w[e] = 0;
           }
@@ -440,7 +551,7 @@ struct Row {
 
   // Whatever the settings and the row are: sweeps for the cut by count and by mass (8 bits of the key
   // each), one for the total, and one in index order that ends at the token.
-  __device__ void in_general(u64 count) const
+  __device__ __forceinline__ void in_general(u64 count) const
   {
     u64* bins = box.c.entries;
     // the cut in rank order: every element with a key above `key`, and with it up to index `last`
@@ -450,7 +561,7 @@ struct Row {
     u64 with      = 0;        // how many there are
     const u32 top = key_of<T>(max);
     if (set.top_k > 0 && (u64)set.top_k < count) {
-      const Cut c = find_cut<T, THREADS>(
+      const Cut c = find_cut<T, THREADS, true>(
         row, n, top, (u64)set.top_k, [&](float x, int i) { return (u64)(eligible(x, i) ? 1 : 0); }, bins);
       key  = c.key;
       take = (u64)set.top_k - c.above;
@@ -458,7 +569,7 @@ struct Row {
     }
     if (set.top_p < 1.0f) {
       u64 all = 0;
-      sweep<T, THREADS>(row, n, [&](float x, int i) {
+      narrow_sweep<T, THREADS>(row, n, [&](float x, int i) {
         if (!eligible(x, i)) return;
         const u32 k = key_of<T>(x);
         if (k > key || (k == key && take == ~(u64)0)) all += weight(x);
@@ -467,7 +578,7 @@ struct Row {
       if (take != ~(u64)0) all += take * weight(value_of<T>(key));
       const u64 goal = set.nucleus(all);
       if (goal < all) {
-        const Cut c = find_cut<T, THREADS>(
+        const Cut c = find_cut<T, THREADS, true>(
           row, n, top, goal, [&](float x, int i) { return eligible(x, i) ? weight(x) : (u64)0; }, bins);
         const u64 each = weight(value_of<T>(c.key));
         key            = c.key;
@@ -477,15 +588,15 @@ struct Row {
     }
     if (take < with) {  // where the last of the equal elements is that is kept
       u64 seen = 0;
-      ordered_sweep<T, THREADS>(row, n, [&](int at, const float(&x)[VEC], int cnt) {
+      ordered_sweep<T, THREADS, 2>(row, n, [&](int at, const float(&x)[2], int cnt) {
         u64 ties = 0;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j)
+        for (int j = 0; j < 2; ++j)
           if (j < cnt && key_of<T>(x[j]) == key && eligible(x[j], at + j)) ++ties;
         u64 all;
         u64 rank = seen + block_before<W>(ties, box.box, all);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j)
+        for (int j = 0; j < 2; ++j)
           if (j < cnt && key_of<T>(x[j]) == key && eligible(x[j], at + j) && ++rank == take) box.found[0] = (u64)(at + j);
         seen += all;
         return seen < take;
@@ -501,18 +612,18 @@ struct Row {
       return w >= least ? w : 0;
     };
     u64 all = 0;
-    sweep<T, THREADS>(row, n, [&](float x, int i) { all += kept(x, i); });
+    narrow_sweep<T, THREADS>(row, n, [&](float x, int i) { all += kept(x, i); });
     all            = block_all<W>(all, AddF{}, box.box);
     const u64 goal = set.goal(all);
     u64 seen       = 0;
-    ordered_sweep<T, THREADS>(row, n, [&](int at, const float(&x)[VEC], int cnt) {
-      u64 own[VEC], sum = 0;
+    ordered_sweep<T, THREADS, 2>(row, n, [&](int at, const float(&x)[2], int cnt) {
+      u64 own[2], sum = 0;
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) sum += own[j] = j < cnt ? kept(x[j], at + j) : 0;
+      for (int j = 0; j < 2; ++j) sum += own[j] = j < cnt ? kept(x[j], at + j) : 0;
       u64 tile;
       u64 upto = seen + block_before<W>(sum, box.box, tile);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
+      for (int j = 0; j < 2; ++j) {
         if (upto <= goal && upto + own[j] > goal) answer(at + j, own[j], all);
         upto += own[j];
       }
@@ -542,7 +653,7 @@ __global__ __launch_bounds__(64 * W, 4) void sample_kernel(SampleArgs a)
   const bool sharp  = set.top_k > 0 && set.top_k <= 64 * W;
   const bool some   = set.top_p < 1.0f || set.min_p > 0.0f;
   const bool sum    = !sharp && set.top_p < 1.0f;
-  const int target  = sharp ? set.top_k : (some && set.top_k <= 0 ? 16 * W : 1);
+  const int target  = sharp ? set.top_k : (some && set.top_k <= 0 ? Row<T, W, MASKED>::kNucleus : 1);
   const float c     = (float)(kLog2e / (double)set.temperature);
   Running run;
   const Found f = stream_candidates<T, W, NV, MASKED ? Look::kMasked : Look::kReal, true>(row, n, target, allowed, c, box.c,
@@ -569,14 +680,16 @@ __global__ __launch_bounds__(64 * W, 4) void sample_kernel(SampleArgs a)
     mass = block_all<W>(run.against(f.max, c), AddF{}, reinterpret_cast<double*>(box.box)) * one;
     off  = ((double)n / THREADS + 256.0 + fabs(weight.m * weight.c)) * 0x1p-23;
   }
+  u64 base  = 0;
+  int known = 0;
   if (set.greedy || sharp || (some && set.top_k <= 0))
-    if (it.from_candidates(f, mass, off)) return;
+    if (it.from_candidates(f, mass, off, base, known)) return;
   __syncthreads();
   if (set.top_k <= 0 || set.top_k >= n)
-    if (it.from_segments(mass, off)) return;
+    if (it.from_segments(mass, off, base, known)) return;
   // the general way starts from the number of elements that count
   u64 count = 0;
-  sweep<T, THREADS>(row, n, [&](float x, int i) { count += it.eligible(x, i) ? 1 : 0; });
+  narrow_sweep<T, THREADS>(row, n, [&](float x, int i) { count += it.eligible(x, i) ? 1 : 0; });
   count = block_all<W>(count, AddF{}, box.box);
   it.in_general(count);
 }
@@ -585,8 +698,13 @@ template <class T>
 int launch(const SampleArgs& a, hipStream_t st)
 {
   const dim3 grid = grid_of(a.n_rows);
+  const bool many = a.n_rows > cu_count();
   const bool wide = (int64_t)a.n_cols / In<T>::VEC > 1024;
-  if (wide && a.allowed != nullptr)
+  if (wide && many && a.allowed != nullptr)
+    hipLaunchKernelGGL((sample_kernel<T, 8, 4, true>), grid, dim3(512), 0, st, a);
+  else if (wide && many)
+    hipLaunchKernelGGL((sample_kernel<T, 8, 4, false>), grid, dim3(512), 0, st, a);
+  else if (wide && a.allowed != nullptr)
     hipLaunchKernelGGL((sample_kernel<T, 16, 4, true>), grid, dim3(1024), 0, st, a);
   else if (wide)
     hipLaunchKernelGGL((sample_kernel<T, 16, 4, false>), grid, dim3(1024), 0, st, a);

@@ -18,30 +18,10 @@ struct TopKArgs {
   double inv_t;
 };
 
-// Descending, `size` (a power of two) entries.
-template <int THREADS>
-__device__ __forceinline__ void sort_entries(u64* e, int size)
-{
-  for (int len = 2; len <= size; len <<= 1) {
-    for (int d = len >> 1; d > 0; d >>= 1) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < size / 2; i += THREADS) {
-        const int a = 2 * i - (i & (d - 1));
-        const u64 x = e[a], y = e[a + d];
-        if ((x < y) == ((a & len) == 0)) {
-          e[a]     = y;
-          e[a + d] = x;
-        }
-      }
-    }
-  }
-  __syncthreads();
-}
-
 // What a row's candidates do not fit: the key of the k-th element by sweeps of the row, 8 bits of
 // the key a sweep, then the elements above it and the first ones that have it, in index order.
 template <class T, int W>
-__device__ __noinline__ void gather_exact(const T* row, int n, int k, float max, CandidateBox<W>& box)
+__device__ __forceinline__ void gather_exact(const T* row, int n, int k, float max, CandidateBox<W>& box)
 {
   constexpr int THREADS = 64 * W;
   constexpr int VEC     = In<T>::VEC;
