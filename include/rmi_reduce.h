@@ -362,9 +362,7 @@ RMI_API int rmi_cov(int dtype,
  * rows start `ld` elements apart (ld >= n_cols; what lies between a row's end and the next row is
  * never read or written).  n_cols is below 2^31 - 65536 and n_rows below 2^31; an element's offset
  * may pass 32 bits.  Rows of other element types are refused with RMI_ERR_UNSUPPORTED, a
- * temperature outside [1e-6, 1e6] likewise.  Workspaces follow the rules of rmi_reduce: their
- * contents need no initialisation, their first RMI_WORKSPACE_TICKET_BYTES bytes are left alone,
- * and calls that share one are ordered on one stream.  Results are the same bits every time.
+ * temperature outside [1e-6, 1e6] likewise.  Results are the same bits every time.
  * None of them has a counterpart in the reference. */
 
 /* The k elements of every row that rank first, in rank order: larger values first, NaN behind
@@ -374,7 +372,6 @@ RMI_API int rmi_cov(int dtype,
  * of the whole row; it is NaN for a row that holds NaN, -inf for one of -inf only, and +inf for one that
  * holds +inf.  1 <= k <= n_cols and k <= RMI_TOP_K_MAX, or RMI_ERR_BAD_SHAPE. */
 #define RMI_TOP_K_MAX 1024
-RMI_API size_t rmi_top_k_workspace_bytes(int dtype, int64_t n_rows, int64_t n_cols, int k);
 RMI_API int rmi_top_k(int dtype,
                       int64_t n_rows,
                       int64_t n_cols,
@@ -385,8 +382,6 @@ RMI_API int rmi_top_k(int dtype,
                       void* values,
                       int32_t* indices,
                       float* lse,
-                      void* workspace,
-                      size_t workspace_bytes,
                       void* stream);
 
 /* Distillation: the loss of student logits z against the best logits that a teacher left for every
@@ -400,17 +395,17 @@ RMI_API int rmi_top_k(int dtype,
  *   dz_iv = row_grad[i] * scale / T * (q_iv sum_j p_ij - sum of p_ij over j with t_indices[i][j] = v).
  * scale = T^2 gives the usual weight, T^2 / n_rows the mean over the rows.  row_grad is the gradient
  * that arrives at loss[i]; NULL stands for ones.  A row without a used entry has loss 0 and gradient
- * 0, whatever its logits.  A listed token whose logit is -inf makes the loss +inf.  A NaN or a +inf
- * among the logits makes the row's loss and gradient NaN.  The same token may be listed more than once.
+ * 0, whatever its logits.  A listed token whose logit is -inf makes the loss +inf.  A NaN
+ * among the logits makes the row's loss and gradient NaN, a +inf what the formulas give with a sum of
+ * +inf (q = 0, NaN at the place itself).  Logits that are all -inf have q = 0.  The same token may be listed more than once.
  *
- * rmi_distill_loss writes `loss`, and what the caller asks for of the rest: `stats`[n_rows][2] (the
- * row's maximum and log(sum_v exp((z_v - max) / T)), what rmi_distill_grad wants) and `grad`
+ * rmi_distill_loss writes `loss`, and what the caller asks for of the rest: `stats`[n_rows][2] (a
+ * logit r near the row's maximum and log(sum_v exp((z_v - r) / T)), what rmi_distill_grad wants) and `grad`
  * ([n_rows][n_cols] of dtype, rows ld_grad apart), which then costs one pass over the logits instead
  * of two.  rmi_distill_grad writes `grad` from the stats of an earlier rmi_distill_loss with the same
  * logits, teacher and temperature.  `grad` may be the logits' own memory if ld_grad = ld.
  * 0 <= k <= RMI_DISTILL_MAX. */
 #define RMI_DISTILL_MAX 1024
-RMI_API size_t rmi_distill_workspace_bytes(int dtype, int64_t n_rows, int64_t n_cols, int k);
 RMI_API int rmi_distill_loss(int dtype,
                              int t_dtype,
                              int64_t n_rows,
@@ -428,8 +423,6 @@ RMI_API int rmi_distill_loss(int dtype,
                              const float* row_grad,
                              void* grad,
                              int64_t ld_grad,
-                             void* workspace,
-                             size_t workspace_bytes,
                              void* stream);
 RMI_API int rmi_distill_grad(int dtype,
                              int t_dtype,

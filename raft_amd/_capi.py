@@ -95,14 +95,11 @@ SYMBOLS = {
     "rmi_cov_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int64, C.c_int64]),
     "rmi_cov": (C.c_int, [C.c_int, C.c_int, C.c_int64, C.c_int64, C.c_int, C.c_int, C.c_void_p,
                           C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
-    "rmi_top_k_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int64, C.c_int64, C.c_int]),
     "rmi_top_k": (C.c_int, [C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_int, C.c_double,
-                            C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t,
-                            C.c_void_p]),
-    "rmi_distill_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int64, C.c_int64, C.c_int]),
+                            C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "rmi_distill_loss": (C.c_int, [C.c_int, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_int,
                                    C.c_double, C.c_double] + [C.c_void_p] * 8 +
-                         [C.c_int64, C.c_void_p, C.c_size_t, C.c_void_p]),
+                         [C.c_int64, C.c_void_p]),
     "rmi_distill_grad": (C.c_int, [C.c_int, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_int,
                                    C.c_double, C.c_double] + [C.c_void_p] * 7 +
                          [C.c_int64, C.c_void_p]),

@@ -1,4 +1,4 @@
-// rmi_distill_loss / rmi_distill_grad / rmi_distill_workspace_bytes (include/rmi_reduce.h):
+// rmi_distill_loss / rmi_distill_grad (include/rmi_reduce.h):
 // the loss of a row of student logits against a teacher's stored best logits, and its gradient.
 //
 //   p_j = exp(t_j / T - L),  q_v = exp((z_v - m) / T) / s,  m = max z,  s = sum_v exp((z_v - m) / T)
@@ -707,8 +707,6 @@ int run(int dtype, int t_dtype, int64_t n_rows, int64_t n_cols, int64_t ld, int6
 
 extern "C" {
 
-size_t rmi_distill_workspace_bytes(int, int64_t, int64_t, int) { return 0; }
-
 int rmi_distill_loss(int dtype,
                      int t_dtype,
                      int64_t n_rows,
@@ -726,8 +724,6 @@ int rmi_distill_loss(int dtype,
                      const float* row_grad,
                      void* grad,
                      int64_t ld_grad,
-                     void*,
-                     size_t,
                      void* stream)
 {
   using namespace rmi::logits;

@@ -1,4 +1,4 @@
-// rmi_top_k / rmi_top_k_workspace_bytes (include/rmi_reduce.h): the k elements of every row that
+// rmi_top_k (include/rmi_reduce.h): the k elements of every row that
 // rank first, in rank order, and the row's log-sum-exp.
 #include "rmi_logits.hpp"
 #include "rmi_normalize.hpp"
@@ -142,8 +142,6 @@ int launch(const TopKArgs& a, hipStream_t st)
 
 extern "C" {
 
-size_t rmi_top_k_workspace_bytes(int, int64_t, int64_t, int) { return 0; }
-
 int rmi_top_k(int dtype,
               int64_t n_rows,
               int64_t n_cols,
@@ -154,8 +152,6 @@ int rmi_top_k(int dtype,
               void* values,
               int32_t* indices,
               float* lse,
-              void*,
-              size_t,
               void* stream)
 {
   using namespace rmi;

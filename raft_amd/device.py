@@ -87,6 +87,9 @@ def cov(dtype: int, layout: int, n_rows: int, n_cols: int, sample: bool, data: t
 # ---- rows of logits -------------------------------------------------------------------------------
 
 _LOGITS_DTYPE = {torch.float16: api.F16, torch.bfloat16: api.BF16, torch.float32: api.F32}
+# the address of a device's current stream, without a Stream object around it where torch has that
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _dtype_of(t: torch.Tensor, what: str) -> int:
@@ -101,101 +104,78 @@ def _logits(x: torch.Tensor, what: str = "logits") -> tuple[int, int, int, int]:
     d = _dtype_of(x, what)
     if x.dim() != 2 or not x.is_cuda:
         raise ValueError(f"{what}: a matrix on the GPU is wanted")
-    (n_rows, n_cols), (ld, step) = x.shape, x.stride()
+    n_rows, n_cols = x.shape
+    ld, step = x.stride()
     if step != 1 and n_cols > 1:
         raise ValueError(f"{what}: the elements of a row have to be contiguous")
-    if n_rows > 1 and ld < n_cols:
-        raise ValueError(f"{what}: rows overlap")
-    return d, n_rows, n_cols, max(ld, n_cols)
+    if ld < n_cols:
+        if n_rows > 1:
+            raise ValueError(f"{what}: rows overlap")
+        ld = n_cols
+    return d, n_rows, n_cols, ld
 
 
-def _ptr(t: torch.Tensor | None, shape: tuple, dtype, like: torch.Tensor, what: str) -> int | None:
-    """Address of a contiguous tensor of that shape and type beside `like`; None stays None."""
+def _ptr(t: torch.Tensor | None, shape: tuple, dtype, device: int, what: str) -> int | None:
+    """Address of a contiguous tensor of that shape and type on that GPU; None stays None."""
     if t is None:
         return None
-    if t.dtype != dtype or t.shape != shape or not t.is_contiguous() or t.device != like.device:
-        raise ValueError(f"{what}: a contiguous {dtype} tensor of shape {tuple(shape)} on {like.device} is wanted, "
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{what}: a contiguous {dtype} tensor of shape {tuple(shape)} on GPU {device} is wanted, "
                          f"got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-def _workspace(given: torch.Tensor | None, n: int, like: torch.Tensor) -> tuple[torch.Tensor | None, int | None, int]:
-    if given is None and n > 0:
-        given = torch.empty(n, dtype=torch.uint8, device=like.device)
-    if given is None:
-        return None, None, 0
-    if given.device != like.device:
-        raise ValueError(f"workspace: memory on {like.device} is wanted")
-    return given, given.data_ptr(), given.numel() * given.element_size()
-
-
-class _on:
-    """The device of a tensor made current for a call, and its current stream."""
-
-    def __init__(self, t: torch.Tensor):
-        self.guard = torch.cuda.device(t.device) if t.device.index != torch.cuda.current_device() else None
-        self.stream = torch.cuda.current_stream(t.device).cuda_stream
-
-    def __enter__(self) -> int:
-        if self.guard is not None:
-            self.guard.__enter__()
-        return self.stream
-
-    def __exit__(self, *exc) -> None:
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _call(name: str, device: int, *args) -> None:
+    """The library's call with that device current, on its current stream."""
+    fn = getattr(api.load(), name)
+    if device == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, _raw_stream(device))
+    if rc != api.OK:
+        raise RmiError(rc, name)
 
 
 def top_k(x: torch.Tensor, values: torch.Tensor, indices: torch.Tensor, lse: torch.Tensor | None = None, *,
-          temperature: float = 1.0, workspace: torch.Tensor | None = None) -> None:
+          temperature: float = 1.0) -> None:
     """Run rmi_top_k on the current torch stream: the k = values.shape[1] elements of every row of
     `x` that rank first (int32 `indices`), and log(sum(exp(x / temperature))) of every row."""
-    lib = api.load()
     d, n_rows, n_cols, ld = _logits(x)
-    k = values.shape[-1]
-    vp = _ptr(values, (n_rows, k), x.dtype, x, "values")
-    ip = _ptr(indices, (n_rows, k), torch.int32, x, "indices")
-    lp = _ptr(lse, (n_rows,), torch.float32, x, "lse")
-    with _on(x) as stream:
-        _, wp, wn = _workspace(workspace, lib.rmi_top_k_workspace_bytes(d, n_rows, n_cols, k), x)
-        rc = lib.rmi_top_k(d, n_rows, n_cols, ld, k, temperature, x.data_ptr(), vp, ip, lp, wp, wn, stream)
-    if rc != api.OK:
-        raise RmiError(rc, "rmi_top_k")
+    device, shape = x.get_device(), (n_rows, values.shape[-1])
+    _call("rmi_top_k", device, d, n_rows, n_cols, ld, shape[1], temperature, x.data_ptr(),
+          _ptr(values, shape, x.dtype, device, "values"), _ptr(indices, shape, torch.int32, device, "indices"),
+          _ptr(lse, (n_rows,), torch.float32, device, "lse"))
 
 
-def _teacher(x: torch.Tensor, t_values, t_indices, teacher_lse, row_grad) -> tuple:
-    n_rows, k = x.shape[0], t_values.shape[-1]
-    return (_dtype_of(t_values, "t_values"), k, _ptr(t_values, (n_rows, k), t_values.dtype, x, "t_values"),
-            _ptr(t_indices, (n_rows, k), torch.int32, x, "t_indices"),
-            _ptr(teacher_lse, (n_rows,), torch.float32, x, "teacher_lse"),
-            _ptr(row_grad, (n_rows,), torch.float32, x, "row_grad"))
+def _teacher(n_rows: int, device: int, t_values, t_indices, teacher_lse) -> tuple:
+    shape = (n_rows, t_values.shape[-1])
+    return (_ptr(t_values, shape, t_values.dtype, device, "t_values"),
+            _ptr(t_indices, shape, torch.int32, device, "t_indices"),
+            _ptr(teacher_lse, (n_rows,), torch.float32, device, "teacher_lse"))
 
 
-def _grad(x: torch.Tensor, grad: torch.Tensor) -> tuple[int, int]:
-    if grad.dtype != x.dtype or grad.shape != x.shape or grad.device != x.device:
+def _grad(x: torch.Tensor, grad: torch.Tensor | None) -> tuple[int | None, int]:
+    if grad is None:
+        return None, 0
+    if grad.dtype is not x.dtype or grad.shape != x.shape or grad.get_device() != x.get_device():
         raise ValueError("grad: the type, shape and device of the logits are wanted")
     return grad.data_ptr(), _logits(grad, "grad")[3]
 
 
 def distill_loss(x: torch.Tensor, t_values: torch.Tensor, t_indices: torch.Tensor, loss: torch.Tensor,
                  stats: torch.Tensor | None = None, grad: torch.Tensor | None = None, *, temperature: float = 1.0,
-                 scale: float = 1.0, teacher_lse: torch.Tensor | None = None, row_grad: torch.Tensor | None = None,
-                 workspace: torch.Tensor | None = None) -> None:
+                 scale: float = 1.0, teacher_lse: torch.Tensor | None = None,
+                 row_grad: torch.Tensor | None = None) -> None:
     """Run rmi_distill_loss on the current torch stream: the loss of every row of student logits
     against a teacher's stored best logits; `stats` ([rows, 2]) for distill_grad, or the gradient at
     once in `grad`, which may be `x`."""
-    lib = api.load()
     d, n_rows, n_cols, ld = _logits(x)
-    td, k, tv, ti, tl, rg = _teacher(x, t_values, t_indices, teacher_lse, row_grad)
-    lp = _ptr(loss, (n_rows,), torch.float32, x, "loss")
-    sp = _ptr(stats, (n_rows, 2), torch.float32, x, "stats")
-    gp, ldg = _grad(x, grad) if grad is not None else (None, 0)
-    with _on(x) as stream:
-        _, wp, wn = _workspace(workspace, lib.rmi_distill_workspace_bytes(d, n_rows, n_cols, k), x)
-        rc = lib.rmi_distill_loss(d, td, n_rows, n_cols, ld, k, temperature, scale, x.data_ptr(), tv, ti, tl, lp, sp,
-                                  rg, gp, ldg, wp, wn, stream)
-    if rc != api.OK:
-        raise RmiError(rc, "rmi_distill_loss")
+    device = x.get_device()
+    _call("rmi_distill_loss", device, d, _dtype_of(t_values, "t_values"), n_rows, n_cols, ld, t_values.shape[-1],
+          temperature, scale, x.data_ptr(), *_teacher(n_rows, device, t_values, t_indices, teacher_lse),
+          _ptr(loss, (n_rows,), torch.float32, device, "loss"), _ptr(stats, (n_rows, 2), torch.float32, device, "stats"),
+          _ptr(row_grad, (n_rows,), torch.float32, device, "row_grad"), *_grad(x, grad))
 
 
 def distill_grad(x: torch.Tensor, t_values: torch.Tensor, t_indices: torch.Tensor, stats: torch.Tensor,
@@ -203,16 +183,12 @@ def distill_grad(x: torch.Tensor, t_values: torch.Tensor, t_indices: torch.Tenso
                  teacher_lse: torch.Tensor | None = None, row_grad: torch.Tensor | None = None) -> None:
     """Run rmi_distill_grad on the current torch stream: the gradient of an earlier distill_loss from
     its `stats`, for the gradient `row_grad` of every row's loss (None: ones)."""
-    lib = api.load()
     d, n_rows, n_cols, ld = _logits(x)
-    td, k, tv, ti, tl, rg = _teacher(x, t_values, t_indices, teacher_lse, row_grad)
-    sp = _ptr(stats, (n_rows, 2), torch.float32, x, "stats")
-    gp, ldg = _grad(x, grad)
-    with _on(x) as stream:
-        rc = lib.rmi_distill_grad(d, td, n_rows, n_cols, ld, k, temperature, scale, x.data_ptr(), tv, ti, tl, sp, rg,
-                                  gp, ldg, stream)
-    if rc != api.OK:
-        raise RmiError(rc, "rmi_distill_grad")
+    device = x.get_device()
+    _call("rmi_distill_grad", device, d, _dtype_of(t_values, "t_values"), n_rows, n_cols, ld, t_values.shape[-1],
+          temperature, scale, x.data_ptr(), *_teacher(n_rows, device, t_values, t_indices, teacher_lse),
+          _ptr(stats, (n_rows, 2), torch.float32, device, "stats"),
+          _ptr(row_grad, (n_rows,), torch.float32, device, "row_grad"), *_grad(x, grad))
 
 
 def sample(x: torch.Tensor, u: torch.Tensor, token: torch.Tensor, logprob: torch.Tensor | None = None, *,
@@ -221,24 +197,25 @@ def sample(x: torch.Tensor, u: torch.Tensor, token: torch.Tensor, logprob: torch
            allowed: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> None:
     """Run rmi_sample on the current torch stream: one int32 `token` of every row of `x` for the
     random numbers `u`, with one setting per row (`top_k` int32, the others float32), and among the
-    tokens whose bit is set in `allowed` ([rows, ceil(vocabulary / 32)] int32 or uint32 words)."""
-    lib = api.load()
+    tokens whose bit is set in `allowed` ([rows, ceil(vocabulary / 32)] int32 or uint32 words).
+    `workspace`: bytes that a caller keeps for it (rmi_sample_workspace_bytes), else allocated here."""
     d, n_rows, n_cols, ld = _logits(x)
-    per_row = (n_rows,)
+    device, rows, f32 = x.get_device(), (n_rows,), torch.float32
     ap, lda = None, 0
     if allowed is not None:
         words = (n_cols + 31) // 32
         if (allowed.dtype not in (torch.int32, torch.uint32) or allowed.shape != (n_rows, words)
                 or (allowed.stride(1) != 1 and words > 1) or (n_rows > 1 and allowed.stride(0) < words)
-                or allowed.device != x.device):
-            raise ValueError(f"allowed: [{n_rows}, {words}] 32-bit words on {x.device} are wanted")
+                or allowed.get_device() != device):
+            raise ValueError(f"allowed: [{n_rows}, {words}] 32-bit words on GPU {device} are wanted")
         ap, lda = allowed.data_ptr(), max(allowed.stride(0), words)
-    args = (_ptr(temperature, per_row, torch.float32, x, "temperature"), _ptr(top_k, per_row, torch.int32, x, "top_k"),
-            _ptr(top_p, per_row, torch.float32, x, "top_p"), _ptr(min_p, per_row, torch.float32, x, "min_p"),
-            _ptr(u, per_row, torch.float32, x, "u"), _ptr(token, per_row, torch.int32, x, "token"),
-            _ptr(logprob, per_row, torch.float32, x, "logprob"))
-    with _on(x) as stream:
-        _, wp, wn = _workspace(workspace, lib.rmi_sample_workspace_bytes(d, n_rows, n_cols), x)
-        rc = lib.rmi_sample(d, n_rows, n_cols, ld, x.data_ptr(), ap, lda, *args, wp, wn, stream)
-    if rc != api.OK:
-        raise RmiError(rc, "rmi_sample")
+    if workspace is None:
+        n = api.load().rmi_sample_workspace_bytes(d, n_rows, n_cols)
+        workspace = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+    elif workspace.get_device() != device:
+        raise ValueError(f"workspace: memory on GPU {device} is wanted")
+    wp, wn = (workspace.data_ptr(), workspace.nbytes) if workspace is not None else (None, 0)
+    _call("rmi_sample", device, d, n_rows, n_cols, ld, x.data_ptr(), ap, lda,
+          _ptr(temperature, rows, f32, device, "temperature"), _ptr(top_k, rows, torch.int32, device, "top_k"),
+          _ptr(top_p, rows, f32, device, "top_p"), _ptr(min_p, rows, f32, device, "min_p"), _ptr(u, rows, f32, device, "u"),
+          _ptr(token, rows, torch.int32, device, "token"), _ptr(logprob, rows, f32, device, "logprob"), wp, wn)

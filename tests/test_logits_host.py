@@ -11,10 +11,10 @@ def _call(name, change):
     lib = api.load()
     args = {
         "rmi_top_k": dict(dtype=api.F32, n_rows=2, n_cols=100, ld=100, k=5, temperature=1.0, logits=P, values=P,
-                          indices=P, lse=P, ws=None, ws_bytes=0, stream=None),
+                          indices=P, lse=P, stream=None),
         "rmi_distill_loss": dict(dtype=api.F32, t_dtype=api.F32, n_rows=2, n_cols=100, ld=100, k=5, temperature=1.0,
                                  scale=1.0, logits=P, t_values=P, t_indices=P, t_lse=P, loss=P, stats=P, row_grad=P,
-                                 grad=P, ld_grad=100, ws=None, ws_bytes=0, stream=None),
+                                 grad=P, ld_grad=100, stream=None),
         "rmi_distill_grad": dict(dtype=api.F32, t_dtype=api.F32, n_rows=2, n_cols=100, ld=100, k=5, temperature=1.0,
                                  scale=1.0, logits=P, t_values=P, t_indices=P, t_lse=P, stats=P, row_grad=P, grad=P,
                                  ld_grad=100, stream=None),
@@ -103,9 +103,9 @@ def test_sample_refusals(change, status):
 
 def test_workspace_queries_of_bad_shapes():
     lib = api.load()
-    assert lib.rmi_top_k_workspace_bytes(api.F64, 4, 1 << 20, 8) == 0
-    assert lib.rmi_top_k_workspace_bytes(api.F32, -4, 1 << 20, 8) == 0
-    assert lib.rmi_distill_workspace_bytes(99, 4, 1 << 20, 8) == 0
+    assert lib.rmi_sample_workspace_bytes(api.F64, 400, 1 << 20) == 0
+    assert lib.rmi_sample_workspace_bytes(99, 400, 1 << 20) == 0
+    assert lib.rmi_sample_workspace_bytes(api.F32, -4, 1 << 20) == 0
     assert lib.rmi_sample_workspace_bytes(api.F32, 4, -1) == 0
 
 
