@@ -456,7 +456,9 @@ RMI_API int rmi_distill_grad(int dtype,
  * NULL, gets the log of the token's share of what is left.  A row with nothing to choose from (also
  * n_cols = 0) gets token -1 and logprob -inf.  The weights exp((x - max) / T) are held as whole
  * multiples of 2^-(62 - ceil(log2(n_cols))), at most 2^-50, of the largest one, so that all sums of them are
- * exact; tokens of less weight than half of that are never chosen. */
+ * exact; tokens of less weight than half of that are never chosen.  The workspace follows the rules of
+ * rmi_reduce: rmi_sample_workspace_bytes bytes, 16-byte aligned, no initialisation needed, its first
+ * RMI_WORKSPACE_TICKET_BYTES bytes left alone; calls that share one are ordered on one stream. */
 RMI_API size_t rmi_sample_workspace_bytes(int dtype, int64_t n_rows, int64_t n_cols);
 RMI_API int rmi_sample(int dtype,
                        int64_t n_rows,

@@ -21,6 +21,16 @@ struct SampleArgs {
   int64_t ld, ld_allowed;
   int n_rows, n_cols;
   int bits;  // the weight of the row's maximum is 2^bits
+  struct Undecided* rest;
+  int32_t* todo;  // whether a row is left to the second kernel
+};
+
+// What the first kernel leaves of a row that it could not decide.
+struct Undecided {
+  u64 base;          // exact mass of the first `known` bins
+  double mass, off;  // the row's mass in fp32 and how far it may be off
+  float max;
+  int known;
 };
 
 // exp((x - m) / T) as a whole number of 2^-bits: sums of such weights do not depend on how a row
@@ -94,7 +104,6 @@ struct Settings {
 // What a workgroup keeps in LDS.
 template <int W>
 struct SampleBox {
-  static constexpr int kBinsOfT  = 1024 * W;  // of the distance from the maximum, in log2
   static constexpr int kSegments = 64 * W;
   CandidateBox<W> c;                          // its entries and hits make room for the bins
   u64 sorted[kSegments];                      // candidates in rank order; later the sums of the segments
@@ -108,10 +117,11 @@ struct SampleBox {
   int window[3];
 };
 
-// One row of a workgroup of W waves.
-template <class T, int W, bool MASKED>
+// One row of a workgroup of W waves; W_REST: those of the second kernel, which sets the width of the bins.
+template <class T, int W, int W_REST, bool MASKED>
 struct Row {
   static constexpr int THREADS = 64 * W;
+  static constexpr int BINS    = 1024 * W_REST;  // of the distance from the maximum, in log2
   static constexpr int VEC     = In<T>::VEC;
   const SampleArgs& a;
   const T* row;
@@ -189,20 +199,20 @@ struct Row {
     __syncthreads();
   }
 
-  // The distance of an element from the maximum in parts of 48 / kBinsOfT powers of two.
+  // The distance of an element from the maximum in parts of 48 / BINS powers of two.
   struct Bin {
     float c, r;
     // 0 for the maximum, and larger behind it
     __device__ __forceinline__ float place(float x) const
     {
-      return fminf(fmaxf(fmaf(x, -c, r), 0.0f), (float)(SampleBox<W>::kBinsOfT - 1));
+      return fminf(fmaxf(fmaf(x, -c, r), 0.0f), (float)(BINS - 1));
     }
     __device__ __forceinline__ int operator()(float x) const { return (int)place(x); }
   };
 
   __device__ __forceinline__ Bin bins() const
   {
-    const float per = (float)SampleBox<W>::kBinsOfT / 48.0f;
+    const float per = (float)BINS / 48.0f;
     return Bin{(float)weight.c * per, (float)(weight.m * weight.c) * per};
   }
 
@@ -366,7 +376,6 @@ struct Row {
     const int tid = (int)threadIdx.x, lane = tid & 63;
     const int segments = (n + kSegment - 1) / kSegment;
     if (segments > SampleBox<W>::kSegments || weight.infinite) return false;
-    constexpr int BINS = SampleBox<W>::kBinsOfT;
     const Bin bin      = bins();
     const bool nucleus = set.top_p < 1.0f;
     // what is kept whole, and what may be kept: values from here on (NaN: none)
@@ -633,9 +642,41 @@ struct Row {
   }
 };
 
+template <class T, int W, int W_REST, bool MASKED>
+__device__ __forceinline__ Row<T, W, W_REST, MASKED> row_of(const SampleArgs& a, int64_t r, SampleBox<W>& box,
+                                                            const Settings& set, float max)
+{
+  Weights weight;
+  weight.table    = box.table;
+  weight.m        = (double)max;
+  weight.c        = kLog2e / (double)set.temperature;
+  weight.bits     = a.bits;
+  weight.infinite = max == kInf;
+  const u64 least = (u64)ceil((double)set.min_p * (double)((u64)1 << a.bits));
+  return Row<T, W, W_REST, MASKED>{a, static_cast<const T*>(a.logits) + r * a.ld,
+                                   MASKED ? a.allowed + r * a.ld_allowed : nullptr, box, set, weight, a.n_cols, max, least, r};
+}
+
+// A row that its candidates did not decide.
+template <class T, int W, bool MASKED>
+__device__ __forceinline__ void rest_of_row(const SampleArgs& a, const Settings& set, const Row<T, W, W, MASKED>& it,
+                                            SampleBox<W>& box, const Undecided& rest)
+{
+  if (set.top_k <= 0 || set.top_k >= a.n_cols)
+    if (it.from_segments(rest.mass, rest.off, rest.base, rest.known)) return;
+  // the general way starts from the number of elements that count
+  __syncthreads();
+  u64 count = 0;
+  narrow_sweep<T, 64 * W>(it.row, a.n_cols, [&](float x, int i) { count += it.eligible(x, i) ? 1 : 0; });
+  count = block_all<W>(count, AddF{}, box.box);
+  it.in_general(count);
+}
+
 // One workgroup per row.  One pass finds the maximum, the elements that rank first and, where a nucleus is
-// asked for, the mass in fp32; that is enough wherever what is kept lies among some hundred elements.
-template <class T, int W, int NV, bool MASKED>
+// asked for, the mass in fp32; that is enough wherever what is kept lies among some hundred elements.  With SPLIT a row
+// that it does not decide is left to the second kernel, so that rows of 20 us and of 100 us do not take turns on the
+// same CUs, and the pass that is bound by memory holds a third fewer registers.
+template <class T, int W, int NV, int W_REST, bool MASKED, bool SPLIT>
 __global__ __launch_bounds__(64 * W, 4) void sample_kernel(SampleArgs a)
 {
   constexpr int THREADS = 64 * W;
@@ -645,73 +686,110 @@ __global__ __launch_bounds__(64 * W, 4) void sample_kernel(SampleArgs a)
   if (r >= a.n_rows) return;
   const int tid = (int)threadIdx.x;
   const int n   = a.n_cols;
-  const T* row  = static_cast<const T*>(a.logits) + r * a.ld;
-  const u32* allowed = MASKED ? a.allowed + r * a.ld_allowed : nullptr;
   const Settings set(a, r);
   for (int i = tid; i < kTable; i += THREADS) box.table[i] = exp2((double)i / kTable);
 
   const bool sharp  = set.top_k > 0 && set.top_k <= 64 * W;
   const bool some   = set.top_p < 1.0f || set.min_p > 0.0f;
   const bool sum    = !sharp && set.top_p < 1.0f;
-  const int target  = sharp ? set.top_k : (some && set.top_k <= 0 ? Row<T, W, MASKED>::kNucleus : 1);
+  const bool ranked = sharp || (some && set.top_k <= 0);
+  const int target  = sharp ? set.top_k : (ranked ? Row<T, W, W_REST, MASKED>::kNucleus : 1);
   const float c     = (float)(kLog2e / (double)set.temperature);
   Running run;
-  const Found f = stream_candidates<T, W, NV, MASKED ? Look::kMasked : Look::kReal, true>(row, n, target, allowed, c, box.c,
-                                                                                           run, sum);
+  const Found f = stream_candidates<T, W, NV, MASKED ? Look::kMasked : Look::kReal, true>(
+    static_cast<const T*>(a.logits) + r * a.ld, n, target, MASKED ? a.allowed + r * a.ld_allowed : nullptr, c, box.c, run, sum);
   if (!(f.max > -kInf)) {  // nothing to choose from
     if (tid == 0) {
+      if (SPLIT) a.todo[r] = 0;
       a.token[r] = -1;
       if (a.logprob != nullptr) a.logprob[r] = -kInf;
     }
     return;
   }
-  Weights weight;
-  weight.table    = box.table;
-  weight.m        = (double)f.max;
-  weight.c        = kLog2e / (double)set.temperature;
-  weight.bits     = a.bits;
-  weight.infinite = f.max == kInf;
-  const double one = (double)((u64)1 << a.bits);
-  const Row<T, W, MASKED> it{a, row, allowed, box, set, weight, n, f.max, (u64)ceil((double)set.min_p * one), r};
+  const auto it = row_of<T, W, W_REST, MASKED>(a, r, box, set, f.max);
   // The mass in fp32, and how far it may be off: n / THREADS additions in order and some 64 roundings of a term,
   // as for a log-sum-exp, and the rounding of the reference that the terms are taken against; doubled.
-  double mass = 0, off = 0;
+  Undecided rest{0, 0.0, 0.0, f.max, 0};
   if (sum) {
-    mass = block_all<W>(run.against(f.max, c), AddF{}, reinterpret_cast<double*>(box.box)) * one;
-    off  = ((double)n / THREADS + 256.0 + fabs(weight.m * weight.c)) * 0x1p-23;
+    rest.mass = block_all<W>(run.against(f.max, c), AddF{}, reinterpret_cast<double*>(box.box)) * (double)((u64)1 << a.bits);
+    rest.off  = ((double)n / THREADS + 256.0 + fabs(it.weight.m * it.weight.c)) * 0x1p-23;
   }
-  u64 base  = 0;
-  int known = 0;
-  if (set.greedy || sharp || (some && set.top_k <= 0))
-    if (it.from_candidates(f, mass, off, base, known)) return;
+  const bool done = ranked && it.from_candidates(f, rest.mass, rest.off, rest.base, rest.known);
+  if constexpr (SPLIT) {
+    if (tid != 0) return;
+    a.todo[r] = done ? 0 : 1;
+    if (!done) a.rest[r] = rest;
+  } else {
+    if (done) return;
+    __syncthreads();
+    rest_of_row<T, W, MASKED>(a, set, it, box, rest);
+  }
+}
+
+// The rows that are left: workgroup b takes the b-th of them, which it counts out itself.  Workgroups are dealt to
+// the CUs in order, so by their own numbers the rows that are left would meet on some CUs while others had none (1024 x
+// 131072 f16, 237 rows left: 139 us, counted out 80).  Without COUNTED, which is for so many rows that they even out,
+// it takes its own row.
+template <class T, int W, bool MASKED, bool COUNTED>
+__global__ __launch_bounds__(64 * W, 4) void sample_rest_kernel(SampleArgs a)
+{
+  constexpr int THREADS = 64 * W;
+  __shared__ SampleBox<W> box;
+  const int tid = (int)threadIdx.x;
+  int64_t r     = block_of_grid();
+  if constexpr (COUNTED) {
+    int skip = (int)r;  // rows left that come before the one wanted
+    int base = 0, all = 0, before = 0, left = 0;
+    for (; base < a.n_rows; base += THREADS) {
+      left   = base + tid < a.n_rows ? (a.todo[base + tid] != 0 ? 1 : 0) : 0;
+      before = block_before<W>(left, box.ibox, all);
+      if (all > skip) break;  // the same in every thread
+      skip -= all;
+    }
+    if (base >= a.n_rows) return;
+    if (left != 0 && before == skip) box.window[2] = base + tid;
+    __syncthreads();
+    r = box.window[2];
+  } else {
+    if (r >= a.n_rows || a.todo[r] == 0) return;
+  }
+  for (int i = tid; i < kTable; i += THREADS) box.table[i] = exp2((double)i / kTable);
   __syncthreads();
-  if (set.top_k <= 0 || set.top_k >= n)
-    if (it.from_segments(mass, off, base, known)) return;
-  // the general way starts from the number of elements that count
-  u64 count = 0;
-  narrow_sweep<T, THREADS>(row, n, [&](float x, int i) { count += it.eligible(x, i) ? 1 : 0; });
-  count = block_all<W>(count, AddF{}, box.box);
-  it.in_general(count);
+  const Undecided rest = a.rest[r];
+  const Settings set(a, r);
+  rest_of_row<T, W, MASKED>(a, set, row_of<T, W, W, MASKED>(a, r, box, set, rest.max), box, rest);
+}
+
+constexpr int kCounted = 8192;
+
+template <class T, bool MASKED>
+void launch_as(const SampleArgs& a, hipStream_t st)
+{
+  const dim3 grid = grid_of(a.n_rows);
+  if ((int64_t)a.n_cols / In<T>::VEC <= 1024) {
+    hipLaunchKernelGGL((sample_kernel<T, 4, 4, 4, MASKED, false>), grid, dim3(256), 0, st, a);
+  } else if (a.n_rows <= cu_count()) {
+    // every row has a CU: it wants all the loads that a CU can have in flight, and a second kernel would only wait
+    // for the slowest row of the first (256 x 131072 bf16, every kind of row: 93 us, in two kernels 104)
+    hipLaunchKernelGGL((sample_kernel<T, 16, 4, 16, MASKED, false>), grid, dim3(1024), 0, st, a);
+  } else {
+    // Two rows at a time on a CU hide each other's steps, and the few that their candidates do not decide, which
+    // take many times as long, are dealt out anew (1024 x 131072 f16, nucleus: 153 us, in one kernel 199).
+    hipLaunchKernelGGL((sample_kernel<T, 8, 4, 16, MASKED, true>), grid, dim3(512), 0, st, a);
+    if (a.n_rows <= kCounted)
+      hipLaunchKernelGGL((sample_rest_kernel<T, 16, MASKED, true>), grid, dim3(1024), 0, st, a);
+    else
+      hipLaunchKernelGGL((sample_rest_kernel<T, 16, MASKED, false>), grid, dim3(1024), 0, st, a);
+  }
 }
 
 template <class T>
 int launch(const SampleArgs& a, hipStream_t st)
 {
-  const dim3 grid = grid_of(a.n_rows);
-  const bool many = a.n_rows > cu_count();
-  const bool wide = (int64_t)a.n_cols / In<T>::VEC > 1024;
-  if (wide && many && a.allowed != nullptr)
-    hipLaunchKernelGGL((sample_kernel<T, 8, 4, true>), grid, dim3(512), 0, st, a);
-  else if (wide && many)
-    hipLaunchKernelGGL((sample_kernel<T, 8, 4, false>), grid, dim3(512), 0, st, a);
-  else if (wide && a.allowed != nullptr)
-    hipLaunchKernelGGL((sample_kernel<T, 16, 4, true>), grid, dim3(1024), 0, st, a);
-  else if (wide)
-    hipLaunchKernelGGL((sample_kernel<T, 16, 4, false>), grid, dim3(1024), 0, st, a);
-  else if (a.allowed != nullptr)
-    hipLaunchKernelGGL((sample_kernel<T, 4, 4, true>), grid, dim3(256), 0, st, a);
+  if (a.allowed != nullptr)
+    launch_as<T, true>(a, st);
   else
-    hipLaunchKernelGGL((sample_kernel<T, 4, 4, false>), grid, dim3(256), 0, st, a);
+    launch_as<T, false>(a, st);
   return hipGetLastError() == hipSuccess ? RMI_OK : RMI_ERR_LAUNCH;
 }
 
@@ -721,7 +799,12 @@ int launch(const SampleArgs& a, hipStream_t st)
 
 extern "C" {
 
-size_t rmi_sample_workspace_bytes(int, int64_t, int64_t) { return 0; }
+size_t rmi_sample_workspace_bytes(int dtype, int64_t n_rows, int64_t n_cols)
+{
+  using namespace rmi::logits;
+  if (!is_logits_dtype(dtype) || check_shape(n_rows, n_cols, n_cols) != RMI_OK || n_rows == 0) return 0;
+  return RMI_WORKSPACE_TICKET_BYTES + (size_t)n_rows * (sizeof(Undecided) + sizeof(int32_t));
+}
 
 int rmi_sample(int dtype,
                int64_t n_rows,
@@ -737,8 +820,8 @@ int rmi_sample(int dtype,
                const float* u,
                int32_t* token,
                float* logprob,
-               void*,
-               size_t,
+               void* workspace,
+               size_t workspace_bytes,
                void* stream)
 {
   using namespace rmi;
@@ -754,9 +837,14 @@ int rmi_sample(int dtype,
       !rmi::logits::aligned(min_p, 4) || !rmi::logits::aligned(u, 4) || !rmi::logits::aligned(token, 4) ||
       !rmi::logits::aligned(logprob, 4))
     return RMI_ERR_ALIGNMENT;
+  if (workspace == nullptr || workspace_bytes < rmi_sample_workspace_bytes(dtype, n_rows, n_cols) ||
+      !rmi::logits::aligned(workspace, 16))
+    return RMI_ERR_WORKSPACE;
   SampleArgs a{};
+  a.rest        = reinterpret_cast<Undecided*>(static_cast<char*>(workspace) + RMI_WORKSPACE_TICKET_BYTES);
   a.logits      = logits;
   a.allowed     = allowed;
+  a.todo        = reinterpret_cast<int32_t*>(a.rest + n_rows);
   a.temperature = temperature;
   a.top_k       = top_k;
   a.top_p       = top_p;

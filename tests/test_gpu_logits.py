@@ -444,6 +444,37 @@ def test_sample_long_rows(gpu, dtype, rows, n, spread):
         _check_sample(view, rng.random(rows), rng.random((rows, n)) < 0.2, top_p=rng.random(rows), min_p=0.1 * rng.random(rows))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("times", [5, 140])
+def test_sample_a_row_does_not_depend_on_the_others(gpu, dtype, masked, times):
+    """The same 60 rows of every setting once and many times over: more rows than CUs, then more than
+    8192, of which most need more than one pass."""
+    import torch
+
+    from raft_amd import device
+    rng = np.random.default_rng(times)
+    rows, n = 60, 8200
+    x = rng.normal(0, 0.3, (rows, n))
+    x[7] = -INF
+    view, _ = _put(x, dtype)
+    u, settings = rng.random(rows), _settings(rng, rows, n)
+    allowed = rng.random((rows, n)) < 0.5 if masked else None
+    _check_sample(view, u, allowed, **settings)
+    got = []
+    for count in (1, times):
+        kw = {k: torch.as_tensor(v.astype(np.int32 if k == "top_k" else np.float32)).cuda().repeat(count)
+              for k, v in settings.items()}
+        if masked:
+            kw["allowed"] = torch.as_tensor(L.pack_bits(allowed)).cuda().repeat(count, 1)
+        token = torch.full((rows * count,), -9, dtype=torch.int32, device="cuda")
+        logprob = torch.full((rows * count,), 5.0, device="cuda")
+        device.sample(view.repeat(count, 1), torch.as_tensor(u.astype(np.float32)).cuda().repeat(count), token, logprob, **kw)
+        got.append((token.cpu().numpy(), logprob.cpu().numpy()))
+    for once, many in zip(*got):
+        np.testing.assert_array_equal(np.tile(once, times), many)
+
+
 def test_sample_follows_the_distribution(gpu):
     """One row with many random numbers: the counts of the tokens against their probabilities.  A count
     of N p is off by sqrt(N p) on average; six of those and one are allowed."""

@@ -19,7 +19,7 @@ def _call(name, change):
                                  scale=1.0, logits=P, t_values=P, t_indices=P, t_lse=P, stats=P, row_grad=P, grad=P,
                                  ld_grad=100, stream=None),
         "rmi_sample": dict(dtype=api.F32, n_rows=2, n_cols=100, ld=100, logits=P, allowed=P, ld_allowed=4,
-                           temperature=P, top_k=P, top_p=P, min_p=P, u=P, token=P, logprob=P, ws=None, ws_bytes=0,
+                           temperature=P, top_k=P, top_p=P, min_p=P, u=P, token=P, logprob=P, ws=P, ws_bytes=1 << 20,
                            stream=None),
     }[name]
     assert set(change) <= set(args)
@@ -95,6 +95,7 @@ def test_distill_refusals_of_one_call():
     (dict(top_k=P + 1), api.ERR_ALIGNMENT), (dict(top_p=P + 2), api.ERR_ALIGNMENT),
     (dict(min_p=P + 2), api.ERR_ALIGNMENT), (dict(u=P + 2), api.ERR_ALIGNMENT),
     (dict(token=P + 2), api.ERR_ALIGNMENT), (dict(logprob=P + 2), api.ERR_ALIGNMENT),
+    (dict(ws=None), api.ERR_WORKSPACE), (dict(ws_bytes=65536 + 71), api.ERR_WORKSPACE), (dict(ws=P + 8), api.ERR_WORKSPACE),
     (dict(n_rows=0, logits=None, u=None, token=None), api.OK),
 ])
 def test_sample_refusals(change, status):
