@@ -530,9 +530,9 @@ struct Running {
 template <int THREADS>
 __device__ __forceinline__ void sort_entries(u64* e, int size)
 {
+  __syncthreads();
   for (int len = 2; len <= size; len <<= 1) {
     for (int d = len >> 1; d > 0; d >>= 1) {
-      __syncthreads();
       for (int i = threadIdx.x; i < size / 2; i += THREADS) {
         const int a = 2 * i - (i & (d - 1));
         const u64 x = e[a], y = e[a + d];
@@ -541,9 +541,45 @@ __device__ __forceinline__ void sort_entries(u64* e, int size)
           e[a + d] = x;
         }
       }
+      // Where partners are at most 64 apart, now and in the next step, a wave's 64 pairs are the same 128 entries
+      // again, and its own accesses are in order.
+      if (d > 64 || (d == 1 && len > 64)) {
+        __syncthreads();
+      } else {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+      }
     }
   }
   __syncthreads();
+}
+
+// The same with one entry in every thread's register (`size` at most THREADS, at least 64; threads from `size` on
+// bring nothing and get nothing): partners in one wave meet by a permute, the others in `e`.
+template <int THREADS>
+__device__ __forceinline__ u64 sort_one_each(u64 own, int size, u64* e)
+{
+  const int tid = (int)threadIdx.x;
+  for (int len = 2; len <= size; len <<= 1) {
+    const bool falls = (tid & len) == 0;
+    for (int d = len >> 1; d > 0; d >>= 1) {
+      u64 other;
+      if (d >= 64) {
+        if (tid < size) e[tid] = own;
+        __syncthreads();
+        other = tid < size ? e[tid ^ d] : 0;
+        __syncthreads();
+      } else {
+        const int from = ((tid ^ d) & 63) << 2;
+        const u32 lo   = (u32)__builtin_amdgcn_ds_bpermute(from, (int)(u32)own);
+        const u32 hi   = (u32)__builtin_amdgcn_ds_bpermute(from, (int)(u32)(own >> 32));
+        other          = (u64)hi << 32 | lo;
+      }
+      const bool larger = ((tid & d) == 0) == falls;
+      own               = (own > other) == larger ? own : other;
+    }
+  }
+  return own;
 }
 
 struct Found {

@@ -41,7 +41,7 @@ struct Undecided {
 // The last product adds 2^52, so the rounded weight stands in the low bits of the result.
 constexpr int kTable = 256;
 struct Weights {
-  const double* table;  // 2^(i / 256), in LDS
+  const double* table;  // 2^(bits + i / 256), in LDS
   double m, c;          // t = (x - m) c
   int bits;
   bool infinite;        // the maximum is +inf: whatever else there is weighs nothing
@@ -56,9 +56,7 @@ struct Weights {
     const double f  = t - (up - kRound);
     const int k     = (int)(u32)__builtin_bit_cast(u64, up);
     const double p  = fma(fma(fma(kL3, f, kL2), f, kL), f, 1.0);
-    u64 scaled      = __builtin_bit_cast(u64, table[k & (kTable - 1)]);
-    scaled += (u64)(u32)(((k >> 8) + bits) << 20) << 32;
-    return __builtin_bit_cast(u64, fma(__builtin_bit_cast(double, scaled), p, 4503599627370496.0));
+    return __builtin_bit_cast(u64, fma(__builtin_ldexp(table[k & (kTable - 1)], k >> 8), p, 4503599627370496.0));
   }
   __device__ __forceinline__ u64 operator()(float x) const
   {
@@ -193,9 +191,8 @@ struct Row {
     }
     int size = 512;
     while (size < count) size <<= 1;
-    if (tid >= count && tid < size) box.c.entries[tid] = 0;
-    sort_entries<THREADS>(box.c.entries, size);
-    if (tid < count) box.sorted[tid] = box.c.entries[tid];
+    const u64 own = sort_one_each<THREADS>(tid < count ? box.c.entries[tid] : 0, size, box.sorted);
+    if (tid < count) box.sorted[tid] = own;
     __syncthreads();
   }
 
@@ -236,6 +233,26 @@ struct Row {
     }
     const bool by_k = set.top_k > 0;
     u32 tau        = f.tau;
+    if (!by_k && tau != 0 && set.top_p < 1.0f && set.min_p <= 0.0f) {
+      // a nucleus that is sure to hold more than the candidates needs no order of them.  All values in the bins
+      // before that of tau are candidates.
+      if (!(sum < 1e300) || !(off < 0.01)) return false;
+      const Bin bin = bins();
+      const int end = bin(value_of<float>(tau));
+      u64 mass = 0, inside = 0;
+      for (int i = tid; i < count; i += THREADS) {
+        const float x = value_of<float>(entry_key(box.c.entries[i]));
+        const u64 w   = weight(x);
+        mass += w;
+        inside += bin(x) < end ? w : 0;
+      }
+      mass = block_all<W>(mass, AddF{}, box.box);
+      if ((double)mass < (double)set.top_p * sum * (1 - off)) {
+        base  = block_all<W>(inside, AddF{}, box.box);
+        known = end;
+        return false;
+      }
+    }
     const int target = by_k ? set.top_k : kNucleus;
     if (count > target + target / 4 || count > THREADS) {  // fewer to put in order: one a thread at most
       tau   = thin_out<W>(box.c, count, target, tau, key32(f.max));
@@ -295,12 +312,17 @@ struct Row {
   // The least value whose bin lies before b; NaN if there is none.  Bins fall as values rise.
   __device__ __forceinline__ float least_in(const Bin& bin, int b) const
   {
-    u32 lo = key32(-3.402823466e38f), hi = key32(max);
+    u32 lo = key32(-3.402823466e38f), hi = key32(max);  // hi is one, and what lies before lo is none
     if (bin(max) >= b) return __builtin_nanf("");
-    while (lo < hi) {
-      const u32 mid = lo + (hi - lo) / 2;
-      if (bin(value_of<float>(mid)) < b) hi = mid;
-      else lo = mid + 1;
+    const u32 lane = threadIdx.x & 63;
+    while (lo < hi) {  // 64 places between them at a time, all lanes alike
+      const u32 step = (hi - lo) / 64 + 1;
+      const u32 at   = hi - lo > lane * step ? lo + lane * step : hi;
+      const u64 in   = __ballot(bin(value_of<float>(at)) < b);  // from some lane on
+      const int from = in != 0 ? __builtin_ctzll(in) : 64;
+      const u32 end  = from < 64 && hi - lo > from * step ? lo + from * step : hi;
+      lo             = from > 0 ? lo + (from - 1) * step + 1 : lo;
+      hi             = end;
     }
     return value_of<float>(lo);
   }
@@ -311,7 +333,7 @@ struct Row {
   // A lane's vectors of one segment as they were loaded, with the mask's bits.
   struct Loaded {
     u32x4 w[kVectors];
-    u32 bits[kVectors];
+    u32 bits;  // VEC of every vector
   };
 
   // g(segment, index of the first element, VEC elements) for every vector of the row that this wave has: the
@@ -325,11 +347,12 @@ struct Row {
     const int words = (n + 31) >> 5;
     auto load = [&](int s) {
       Loaded l;
+      l.bits = 0;
 #pragma unroll
       for (int v = 0; v < kVectors; ++v) {
         const int at = s * kSegment + (v * 64 + lane) * VEC;
         l.w[v]       = load16c(row + at);
-        l.bits[v]    = MASKED ? mask_bits(allowed, at, words) : 0;
+        if (MASKED) l.bits |= (mask_bits(allowed, at, words) & ((1u << VEC) - 1)) << (v * VEC);
       }
       return l;
     };
@@ -346,7 +369,7 @@ struct Row {
 #pragma unroll
         for (int v = 0; v < kVectors; ++v) {
           float x[VEC];
-          unpack(now.w[v], now.bits[v], x);
+          unpack(now.w[v], now.bits >> (v * VEC), x);
           g(s, s * kSegment + (v * 64 + lane) * VEC, x);
         }
         now = next;
@@ -397,23 +420,36 @@ struct Row {
       // would be far off for the few heaviest, whose mass is known.
       constexpr int EACH = BINS / THREADS;
       const double one   = (double)((u64)1 << weight.bits);
-      auto mass_of       = [&](int b) {
-        const u32 count = b < known ? 0 : counts[b];
-        return count != 0 ? (double)count * one * (double)__builtin_amdgcn_exp2f(-((float)b + 0.5f) * (48.0f / BINS)) : 0.0;
-      };
+      double mass[EACH];
       double own = 0;
-      for (int e = 0; e < EACH; ++e) own += mass_of(tid * EACH + e);
+      u32 count[EACH];
+#pragma unroll
+      for (int e = 0; e < EACH; e += 4) {
+        const u32x4 four = *reinterpret_cast<const u32x4*>(&counts[tid * EACH + e]);
+#pragma unroll
+        for (int f = 0; f < 4; ++f) count[e + f] = four[f];
+      }
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        const int b   = tid * EACH + e;
+        const float w = __builtin_amdgcn_exp2f(-((float)b + 0.5f) * (48.0f / BINS));
+        mass[e]       = b >= known ? (double)count[e] * ((double)w * one) : 0.0;
+        own += mass[e];
+      }
       double ignored;
       double upto       = (double)base + block_before<W>(own, reinterpret_cast<double*>(box.box), ignored);
       const double goal = (double)set.top_p * sum;
-      // bins are 0.2 or 0.4 % wide, and the places of many values in theirs average out
-      const double give = off + 2e-4;
+      // Bins are 0.2 to 0.8 % wide, and the places of many values in theirs average out: to 1e-5 of the mass where
+      // the values are fine, to 1e-4 and now and then 5e-4 for the few hundred values that bf16 has here.  What
+      // falls short costs three to five times as much as the whole row, some hundred more to put in order 2 us.
+      const double give = off + 5e-4;
       if (tid == 0) box.window[0] = box.window[1] = BINS;
       __syncthreads();
+#pragma unroll
       for (int e = 0; e < EACH; ++e) {
         const int b       = tid * EACH + e;
         const double less = b == 0 ? -1.0 : upto;
-        upto += mass_of(b);
+        upto += mass[e];
         // the first bin that may hold the end, and the first that should lie behind it (one thread each); the
         // exact pass finds out whether that is so
         if (less < goal * (1 - give) && upto >= goal * (1 - give)) box.window[0] = b;
@@ -423,9 +459,10 @@ struct Row {
       // bins before b0 are kept whole, b1 and later ones not at all
       const int b0 = box.window[0] > known ? box.window[0] : known, b1 = box.window[1];
       u32 in = 0;
+#pragma unroll
       for (int e = 0; e < EACH; ++e) {
         const int b = tid * EACH + e;
-        if (b >= b0 && b < b1) in += counts[b];
+        if (b >= b0 && b < b1) in += count[e];
       }
       in = block_all<W>(in, AddF{}, reinterpret_cast<u32*>(box.ibox));
       if (in > (u32)CandidateBox<W>::kEntries) return false;
@@ -435,9 +472,9 @@ struct Row {
     }
     __syncthreads();
 
-    // the exact pass.  Every weight comes with the bits of 2^52; what was added of them is taken off at the end.
+    // the exact pass.  Every weight comes with the bits of 2^52, which are taken off a vector at a time.
     constexpr u64 kHead = 0x4330000000000000ull;
-    u64 all = 0, sum_s = 0, added = 0;
+    u64 all = 0, sum_s = 0;
     int at_segment = -1;
     auto close     = [&]() {  // this wave's segment is complete
       if (at_segment < 0) return;
@@ -445,34 +482,66 @@ struct Row {
       if (lane == 0) box.mass[at_segment] = w;
       sum_s = 0;
     };
-    segments_of_wave([&](int s, int at, const float(&x)[VEC]) {
-      if (s != at_segment) {
-        close();
-        at_segment = s;
-      }
-      u64 w[VEC];
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) w[j] = weight.raw(x[j]);
-      u64 part = 0;
-      if (nucleus) {
+    auto in_segment = [&](int s) {
+      if (s == at_segment) return;
+      close();
+      at_segment = s;
+    };
+    if (nucleus) {
+      segments_of_wave([&](int s, int at, const float(&x)[VEC]) {
+        in_segment(s);
+        u64 part = 0;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          all += w[j];
+          const u64 w     = weight.raw(x[j]);
           const bool kept = x[j] >= above;
-          part += kept ? w[j] : kHead;
-          if (x[j] >= low && !kept)
-            box.c.entries[atomicAdd(&box.c.count, 1)] = entry_of(key32(x[j]), (u32)(at + j));
+          all += w;
+          part += kept ? w : kHead;
         }
-        added += VEC * kHead;
-      } else {
-        const u64 from = least + kHead;
+        all -= VEC * kHead;
+        sum_s += part - VEC * kHead;
+        asm volatile("" : "+v"(sum_s), "+v"(all));  // the sums are formed here, not after the branches
+        // where the values between lie, put down by the wave as a whole: one place is asked for
+        u64 lanes[VEC];
+        int hits = 0;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) part += w[j] >= from ? w[j] : kHead;
-      }
-      sum_s += part - VEC * kHead;
-    });
+        for (int j = 0; j < VEC; ++j) {
+          lanes[j] = __ballot(x[j] >= low && !(x[j] >= above));
+          hits += __builtin_popcountll(lanes[j]);
+        }
+        if (hits == 0) return;
+        int place = 0;
+        if (lane == 0) place = atomicAdd(&box.c.count, hits);
+        place = __builtin_amdgcn_readfirstlane(place);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          if (lanes[j] == 0) continue;
+          const int to = __builtin_amdgcn_mbcnt_hi((u32)(lanes[j] >> 32), __builtin_amdgcn_mbcnt_lo((u32)lanes[j], place));
+          if ((lanes[j] >> lane) & 1) box.c.entries[to] = (u64)(u32)(at + j);
+          place += __builtin_popcountll(lanes[j]);
+        }
+      });
+    } else if (least > 0) {
+      segments_of_wave([&](int s, int, const float(&x)[VEC]) {
+        in_segment(s);
+        u64 part = 0;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const u64 w = weight.raw(x[j]);
+          part += w >= least + kHead ? w : kHead;
+        }
+        sum_s += part - VEC * kHead;
+      });
+    } else {
+      segments_of_wave([&](int s, int, const float(&x)[VEC]) {
+        in_segment(s);
+        u64 part = 0;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) part += weight.raw(x[j]);
+        sum_s += part - VEC * kHead;
+      });
+    }
     close();
-    all -= added;
     __syncthreads();
     u64 total = block_all<W>(tid < segments ? box.mass[tid] : (u64)0, AddF{}, box.box);
     u64 last  = 0;  // the last entry kept of those between b0 and b1
@@ -481,10 +550,20 @@ struct Row {
       const u64 goal = set.nucleus(all);
       const int in   = box.c.count;
       u64* entries   = box.c.entries;
-      int size       = 2;
+      auto entry_at  = [&](int i) {
+        const u32 where = (u32)entries[i];
+        return entry_of(key32(widen(row + where)), where);
+      };
+      int size = 64;
       while (size < in) size <<= 1;
-      for (int i = in + tid; i < size; i += THREADS) entries[i] = 0;
-      sort_entries<THREADS>(entries, size);
+      if (size <= THREADS) {
+        const u64 own = sort_one_each<THREADS>(tid < in ? entry_at(tid) : 0, size, box.sorted);
+        if (tid < in) entries[tid] = own;
+        __syncthreads();
+      } else {
+        for (int i = tid; i < size; i += THREADS) entries[i] = i < in ? entry_at(i) : 0;
+        sort_entries<THREADS>(entries, size);
+      }
       constexpr int EACH = CandidateBox<W>::kEntries / THREADS;  // consecutive ones
       u64 w[EACH], mine = 0;
 #pragma unroll
@@ -677,7 +756,7 @@ __device__ __forceinline__ void rest_of_row(const SampleArgs& a, const Settings&
 // that it does not decide is left to the second kernel, so that rows of 20 us and of 100 us do not take turns on the
 // same CUs, and the pass that is bound by memory holds a third fewer registers.
 template <class T, int W, int NV, int W_REST, bool MASKED, bool SPLIT>
-__global__ __launch_bounds__(64 * W, 4) void sample_kernel(SampleArgs a)
+__global__ __launch_bounds__(64 * W, MASKED && W == 4 ? 3 : 4) void sample_kernel(SampleArgs a)
 {
   constexpr int THREADS = 64 * W;
   __shared__ SampleBox<W> box;
@@ -687,7 +766,7 @@ __global__ __launch_bounds__(64 * W, 4) void sample_kernel(SampleArgs a)
   const int tid = (int)threadIdx.x;
   const int n   = a.n_cols;
   const Settings set(a, r);
-  for (int i = tid; i < kTable; i += THREADS) box.table[i] = exp2((double)i / kTable);
+  for (int i = tid; i < kTable; i += THREADS) box.table[i] = exp2(a.bits + (double)i / kTable);
 
   const bool sharp  = set.top_k > 0 && set.top_k <= 64 * W;
   const bool some   = set.top_p < 1.0f || set.min_p > 0.0f;
@@ -753,7 +832,7 @@ __global__ __launch_bounds__(64 * W, 4) void sample_rest_kernel(SampleArgs a)
   } else {
     if (r >= a.n_rows || a.todo[r] == 0) return;
   }
-  for (int i = tid; i < kTable; i += THREADS) box.table[i] = exp2((double)i / kTable);
+  for (int i = tid; i < kTable; i += THREADS) box.table[i] = exp2(a.bits + (double)i / kTable);
   __syncthreads();
   const Undecided rest = a.rest[r];
   const Settings set(a, r);
