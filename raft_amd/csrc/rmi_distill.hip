@@ -4,6 +4,11 @@
 //   p_j = exp(t_j / T - L),  q_v = exp((z_v - m) / T) / s,  m = max z,  s = sum_v exp((z_v - m) / T)
 //   loss = scale * sum_j p_j (log p_j - (z_{i_j} - m) / T + log s)
 //   dz_v = c * (P q_v - sum_{j: i_j = v} p_j),  c = g * scale / T,  P = sum_j p_j
+//
+// Memory is the bound: with the gradient a row is read once and written once where a workgroup's registers
+// hold it, which is why rows are not split (q needs the whole row's s).  Measured: 4096 x 32000 bf16 100 us (83 at
+// the rate of a copy, 6.5 TB/s); 4096 x 131072 bf16 394 us (332).  In two calls the row is read twice: 1000 x
+// 50001 f32 112 us (90).
 #include "rmi_logits.hpp"
 #include "rmi_normalize.hpp"
 

@@ -475,6 +475,18 @@ def test_sample_a_row_does_not_depend_on_the_others(gpu, dtype, masked, times):
         np.testing.assert_array_equal(np.tile(once, times), many)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,n", [(8, 131072), (300, 9001)])
+def test_sample_top_p_and_min_p(gpu, dtype, rows, n):
+    """Either cut first, and both near one another."""
+    rng = np.random.default_rng(n)
+    view, _ = _put(rng.normal(0, 1.0, (rows, n)), dtype)
+    for min_p in (0.3, 0.05, 0.02, 1e-3):
+        for top_p in (0.02, 0.3, 0.9, 0.999):
+            _check_sample(view[:8], rng.random(8), top_p=np.full(8, top_p), min_p=np.full(8, min_p))
+    _check_sample(view, rng.random(rows), top_p=rng.random(rows), min_p=rng.random(rows) ** 4)
+
+
 def test_sample_follows_the_distribution(gpu):
     """One row with many random numbers: the counts of the tokens against their probabilities.  A count
     of N p is off by sqrt(N p) on average; six of those and one are allowed."""
