@@ -823,7 +823,7 @@ __global__ __launch_bounds__(64 * W, MASKED && W == 4 ? 3 : 4) void sample_kerne
 
 // The rows that are left: workgroup b takes the b-th of them, which it counts out itself.  Workgroups are dealt to
 // the CUs in order, so by their own numbers the rows that are left would meet on some CUs while others had none (1024 x
-// 131072 f16, 237 rows left: 139 us, counted out 80).  Without COUNTED, which is for so many rows that they even out,
+// 131072 f16, 237 rows left: 139 us, counted out 80, and 74 now).  Without COUNTED, which is for so many rows that they even out,
 // it takes its own row.
 template <class T, int W, bool MASKED, bool COUNTED>
 __global__ __launch_bounds__(64 * W, 4) void sample_rest_kernel(SampleArgs a)
@@ -869,7 +869,8 @@ void launch_as(const SampleArgs& a, hipStream_t st)
     hipLaunchKernelGGL((sample_kernel<T, 16, 4, 16, MASKED, false>), grid, dim3(1024), 0, st, a);
   } else {
     // Two rows at a time on a CU hide each other's steps, and the few that their candidates do not decide, which
-    // take many times as long, are dealt out anew (1024 x 131072 f16, nucleus: 153 us, in one kernel 199).
+    // take many times as long, are dealt out anew (1024 x 131072 f16, nucleus, as first built: 153 us, in one kernel
+    // 199; now 146).
     hipLaunchKernelGGL((sample_kernel<T, 8, 4, 16, MASKED, true>), grid, dim3(512), 0, st, a);
     if (a.n_rows <= kCounted)
       hipLaunchKernelGGL((sample_rest_kernel<T, 16, MASKED, true>), grid, dim3(1024), 0, st, a);
