@@ -8,7 +8,7 @@
 // Memory is the bound: with the gradient a row is read once and written once where a workgroup's registers
 // hold it, which is why rows are not split (q needs the whole row's s).  Measured: 4096 x 32000 bf16 100 us (83 at
 // the rate of a copy, 6.5 TB/s); 4096 x 131072 bf16 394 us (332).  In two calls the row is read twice: 1000 x
-// 50001 f32 112 us (90).
+// 50001 f32 108 us (90).
 #include "rmi_logits.hpp"
 #include "rmi_normalize.hpp"
 
@@ -431,10 +431,11 @@ __global__ __launch_bounds__(64 * W, NV > 8 ? 4 : 8) void distill_rows_kernel(Di
 
 // The gradient from the statistics of an earlier forward pass: nothing joins a row's parts, so every
 // workgroup takes one piece of a row, NV vectors a thread, in the order of memory.  (A workgroup that walks
-// a whole row keeps a thousand rows open at once: 1000 x 50001 f32: 92 us against 77.)  Its first wave works the
+// a whole row keeps a thousand rows open at once: 1000 x 50001 f32: 92 us against 77; 72 since it has the registers
+// to spill nothing.)  Its first wave works the
 // teacher's probabilities out again and corrects the listed tokens that lie in the piece.
 template <class T, int W, int NV>
-__global__ __launch_bounds__(64 * W, 6) void distill_grad_kernel(DistillArgs a, int pieces)
+__global__ __launch_bounds__(64 * W, 5) void distill_grad_kernel(DistillArgs a, int pieces)
 {
   constexpr int THREADS = 64 * W;
   constexpr int VEC     = In<T>::VEC;
