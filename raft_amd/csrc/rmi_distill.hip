@@ -431,9 +431,9 @@ __global__ __launch_bounds__(64 * W, NV > 8 ? 4 : 8) void distill_rows_kernel(Di
 
 // The gradient from the statistics of an earlier forward pass: nothing joins a row's parts, so every
 // workgroup takes one piece of a row, NV vectors a thread, in the order of memory.  (A workgroup that walks
-// a whole row keeps a thousand rows open at once: 1000 x 50001 f32: 92 us against 77; 72 since it has the registers
-// to spill nothing.)  Its first wave works the
-// teacher's probabilities out again and corrects the listed tokens that lie in the piece.
+// a whole row keeps a thousand rows open at once: 1000 x 50001 f32: 92 us against 77.  Six
+// waves a SIMD leave it too few registers by five, which costs 4 us.)  Its first wave works the teacher's probabilities
+// out again and corrects the listed tokens that lie in the piece.
 template <class T, int W, int NV>
 __global__ __launch_bounds__(64 * W, 5) void distill_grad_kernel(DistillArgs a, int pieces)
 {
