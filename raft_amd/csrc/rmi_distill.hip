@@ -212,8 +212,9 @@ struct Guess {
   __device__ __forceinline__ void first(const float (&x)[2][V], float ext, float c)
   {
     const float m = max3(max_of(x[0]), max_of(x[1]), ext);
-    run.m         = fabsf(m) < Running::kLarge ? m : 0.0f;
-    run.r         = run.m * c;
+    const float r = product(m, c);
+    run.m         = Running::large(r) ? 0.0f : m;
+    run.r         = Running::large(r) ? 0.0f : r;
   }
   template <int V>
   __device__ __forceinline__ void add(const float (&x)[2][V], float c)
@@ -240,8 +241,8 @@ struct Dense {
   __device__ __forceinline__ Dense(float top, float c_, double factor, double mass, double s) : c(c_)
   {
     ref   = Running::ref(top);
-    r     = ref * c;
-    large = !(fabsf(top) < Running::kLarge);
+    r     = product(ref, c);
+    large = Running::large(r);
     // a row without a finite logit has q = 0 everywhere; without a teacher its gradient is zero
     zero = mass == 0;
     f    = s == 0 || zero ? 0.0f : (float)(factor * mass) / (float)s;
@@ -287,10 +288,7 @@ struct Dense {
 __device__ __forceinline__ double against(float m, double sum, float top, float c)
 {
   if (!(m > -kInf)) return sum;  // nothing, or NaN alone
-  const float q = Running::ref(top) * c;
-  return sum * (double)(fabsf(top) < Running::kLarge && fabsf(m) < Running::kLarge
-                          ? __builtin_amdgcn_exp2f(m * c - q)
-                          : __builtin_amdgcn_exp2f((m - Running::ref(top)) * c));
+  return sum * (double)Running::moved(m, product(Running::ref(m), c), top, product(Running::ref(top), c), c);
 }
 // A wave's maximum and sum into LDS.
 __device__ __forceinline__ void share(const Running& run, float c, float* max, double* sum)
@@ -315,7 +313,8 @@ __device__ __forceinline__ void joined(const float* max, const double* sum, floa
 // What the sum's logarithm belongs to: fl(m c), as a value in units of the logits.
 __device__ __forceinline__ double m_of(float top, const DistillArgs& a)
 {
-  return fabsf(top) < Running::kLarge ? (double)(Running::ref(top) * a.c) * a.ln2_t : (double)Running::ref(top);
+  const float q = product(Running::ref(top), a.c);
+  return Running::large(q) ? (double)Running::ref(top) : (double)q * a.ln2_t;
 }
 __device__ __forceinline__ double factor_of(const DistillArgs& a, int64_t r)
 {

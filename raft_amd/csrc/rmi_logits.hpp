@@ -471,22 +471,41 @@ __device__ __forceinline__ float max_of(const float (&x)[N])
     return max3(max3(x[0], x[1], x[2]), x[3], x[3]);
 }
 
+// a b rounded, always: a product that the compiler joined with a later difference would be another number
+// than the one that terms were taken against.
+__device__ __forceinline__ float product(float a, float b)
+{
+#pragma clang fp contract(off)
+  return a * b;
+}
+
 // A running maximum and sum of exp2((x - m) c) of the elements that one thread sees.  The terms are
 // exp2(fma(x, c, -r)) with r = fl(m c): one rounding each, and r's own drops out of the sum's
-// logarithm, which is taken against r.  Maxima so large that m c overflows (rows of the type's lowest
-// value) take the difference first.
+// logarithm, which is taken against r.  That rounding is in the exponent, 2^-25 of |r| at most: from
+// |r| = 2^17 on, where it reaches 2^-8 (and 128, beyond which nothing is left of a sum, at 2^32), the
+// difference x - m is taken first.
 struct Running {
-  static constexpr float kLarge = 1e30f;
+  static constexpr float kLarge = 0x1p17f;
   float m = -kInf;
-  float r = 0;
+  float r = -kInf;  // nothing yet: the careful way
   float s = 0;
   __device__ __forceinline__ static float ref(float m) { return fabsf(m) < kInf ? m : 0.0f; }
+  // of r = fl(ref(m) c): whether differences are taken first
+  __device__ __forceinline__ static bool large(float r) { return !(fabsf(r) < kLarge); }
+  // What a sum that belongs to m is multiplied by to belong to `to`; r and q are their products with c.
+  __device__ __forceinline__ static float moved(float m, float r, float to, float q, float c)
+  {
+    if (__builtin_expect(!large(fmaxf(fabsf(r), fabsf(q))), 1)) return __builtin_amdgcn_exp2f(r - q);
+    if (!(m > -kInf)) return 1.0f;  // a sum of nothing, or of NaN alone
+    // from r to m c, on to `to` c, and from there to q
+    const float off = (large(q) ? 0.0f : fmaf(ref(to), c, -q)) - (large(r) ? 0.0f : fmaf(ref(m), c, -r));
+    return __builtin_amdgcn_exp2f((ref(m) - ref(to)) * c + off);
+  }
   __device__ __forceinline__ void raise(float to, float c)
   {
     if (to > m) {
-      const float q = ref(to) * c;
-      s *= fabsf(to) < kLarge && fabsf(m) < kLarge ? __builtin_amdgcn_exp2f(r - q)
-                                                   : __builtin_amdgcn_exp2f((m - ref(to)) * c);
+      const float q = product(ref(to), c);
+      s *= moved(m, r, to, q, c);
       m = to;
       r = q;
     }
@@ -496,7 +515,7 @@ struct Running {
   __device__ __forceinline__ void add(const float (&x)[N][V], float c)
   {
     float t[2] = {0, 0};
-    if (__builtin_expect(fabsf(m) < kLarge, 1)) {
+    if (__builtin_expect(!large(r), 1)) {
 #pragma unroll
       for (int i = 0; i < N; ++i)
 #pragma unroll
@@ -510,19 +529,17 @@ struct Running {
     }
     s += t[0] + t[1];
   }
-  // This thread's sum against the maximum `top` of all; top's own r is ref(top) * c.
+  // This thread's sum against the maximum `top` of all; top's own r is fl(ref(top) c).
   __device__ __forceinline__ double against(float top, float c) const
   {
-    const float q = ref(top) * c;
-    if (!(m > -kInf)) return (double)s;  // nothing, or NaN alone
-    return (double)(fabsf(top) < kLarge && fabsf(m) < kLarge ? s * __builtin_amdgcn_exp2f(r - q)
-                                                             : s * __builtin_amdgcn_exp2f((m - ref(top)) * c));
+    return (double)(s * moved(m, r, top, product(ref(top), c), c));
   }
   // log of sum exp(x / T) from all = the sum over the threads of against(top)
   __device__ __forceinline__ static double log_sum(float top, float c, double inv_t, double all)
   {
     if (all == all && fabsf(top) == kInf) return (double)top;
-    return (fabsf(top) < kLarge ? (double)(ref(top) * c) * kLn2 : (double)ref(top) * inv_t) + log(all);
+    const float q = product(ref(top), c);
+    return (large(q) ? (double)ref(top) * inv_t : (double)q * kLn2) + log(all);
   }
 };
 
