@@ -202,11 +202,14 @@ __device__ __forceinline__ void patch(const DistillArgs& a, const TeacherBox& bo
 
 // The sum of exponentials of one thread's elements, two vectors at a time, against the largest of its
 // first two vectors: no maxima after that, which are a third of the instructions.  Any reference gives the
-// sum as long as it neither overflows nor sinks: what a thread's elements say about that is seen in the sum
-// itself, which is at least 1 with a reference out of its own elements.  If it is not, or is not finite, or
+// sum as long as it neither grows much nor sinks: what a thread's elements say about that is seen in the sum
+// itself, which is at least 1 with a reference out of its own elements.  If it is not, or is 2^30 or more, or
 // the reference is too large for one fused step, the thread goes over its elements again and raises the
-// reference as it goes (`again`).
+// reference as it goes.  Below 2^30 the row's maximum is 30 powers of two above the reference at most: exponents
+// keep the precision that the errors of a log-sum-exp are counted with, no thread's sum is lost where a
+// larger reference joins it, and the gradient's factor c P / s stays far from the denormal numbers.
 struct Guess {
+  static constexpr float kMost = 0x1p30f;
   Running run;
   template <int V>
   __device__ __forceinline__ void first(const float (&x)[2][V], float ext, float c)
@@ -226,7 +229,7 @@ struct Guess {
       for (int j = 0; j < V; ++j) t[j & 1] += __builtin_amdgcn_exp2f(fmaf(x[i][j], c, -run.r));
     run.s += t[0] + t[1];
   }
-  __device__ __forceinline__ bool doubtful() const { return !(run.s >= 0.5f && run.s < kInf); }
+  __device__ __forceinline__ bool doubtful() const { return !(run.s >= 0.5f && run.s < kMost); }
 };
 
 // dense part of the gradient: f exp((x - m) / T), f = c P / s

@@ -62,3 +62,37 @@ def test_distill_far_from_zero(gpu, dtype, far, temperature, calls):
     rng = np.random.default_rng(2)
     for n in LENGTHS:
         _distill(_far_rows(far, temperature, n, rng), dtype, temperature, calls, rng)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("temperature", [1.0, 0.25])
+def test_rows_that_begin_far_below_the_rest(gpu, dtype, temperature):
+    """All that a thread sees first lies far below what comes later, or is masked.  A reference taken from it
+    makes the sum of exponentials so large that the gradient's factor sinks below the normal numbers, and then
+    beyond the largest number."""
+    rng = np.random.default_rng(5)
+    per = 4 if dtype == "f32" else 8  # elements of a vector
+    for n in (1000 * per - 5, 4000 * per + 3, 8100 * per, 16300 * per + 1):
+        late = np.arange(n) > 0.9 * n
+        x = []
+        for gap in (15.0, 25.0, 40.0, 60.0, 78.0, 82.0, 86.0, 88.3, 91.0):
+            whole = temperature * rng.normal(0, 1.5, n)
+            whole[late] += gap * temperature       # a whole part lies high
+            one = temperature * rng.normal(0, 1.5, n)
+            one[n - n // 50] = gap * temperature   # a single logit does
+            x += [whole, one]
+        masked = temperature * rng.normal(80, 1.5, n)
+        masked[~late] = -INF
+        x += [masked, np.where(late, rng.normal(21, 0.3, n), -INF)]
+        x = np.array(x)
+        _distill(x, dtype, temperature, 1, rng, scale=1 / 4096)
+        _distill(x, dtype, temperature, 1, rng, scale=1 / 4096, listed=False)
+
+
+def test_many_rows_that_begin_far_below_the_rest(gpu):
+    """The same where workgroups of 8 waves take the rows."""
+    rng = np.random.default_rng(6)
+    rows, n = 520, 12000
+    x = rng.normal(0, 1.5, (rows, n))
+    x[np.arange(rows), n - 1 - np.arange(rows)] = rng.uniform(20, 95, rows)
+    _distill(x, "f32", 1.0, 1, rng, scale=1 / 4096, listed=False)
