@@ -13,8 +13,6 @@
 #include "rmi_normalize.hpp"
 
 namespace rmi {
-int cu_count();  // rmi_api.hip
-
 namespace logits {
 namespace {
 
@@ -32,7 +30,6 @@ struct DistillArgs {
   int t_dtype;
   float c;           // log2(e) / T
   double inv_t, scale;
-  double ln2_t;      // ln(2) T
 };
 
 __device__ __forceinline__ double teacher(const DistillArgs& a, int64_t at)
@@ -168,17 +165,16 @@ __device__ __forceinline__ double loss_of(const DistillArgs& a, const TeacherBox
   return wave_all(loss, AddF{});
 }
 
-__device__ __forceinline__ void write_loss(const DistillArgs& a, const TeacherBox& box, int64_t r, float top, double m,
-                                           double all)
+// s: the sum of exponentials against m = Running::ref(top)
+__device__ __forceinline__ void write_loss(const DistillArgs& a, const TeacherBox& box, int64_t r, float top, double s)
 {
-  const double log_s = log(all);
-  const double loss  = loss_of(a, box, m, log_s);
+  const double log_s = log(s);
+  const double loss  = loss_of(a, box, (double)Running::ref(top), log_s);
   if ((threadIdx.x & 63) != 0) return;
   a.loss[r] = (float)(loss * a.scale);
   if (a.stats != nullptr) {
-    const double ref = (double)Running::ref(top);
-    a.stats[2 * r]     = all == 0 ? -kInf : Running::ref(top);
-    a.stats[2 * r + 1] = (float)(log_s + (m - ref) * a.inv_t);
+    a.stats[2 * r]     = s == 0 ? -kInf : Running::ref(top);
+    a.stats[2 * r + 1] = (float)log_s;
   }
 }
 
@@ -313,12 +309,9 @@ __device__ __forceinline__ void joined(const float* max, const double* sum, floa
   top            = wave_all(m, MaxF{});
   all            = wave_all(against(m, s, top, c), AddF{});
 }
-// What the sum's logarithm belongs to: fl(m c), as a value in units of the logits.
-__device__ __forceinline__ double m_of(float top, const DistillArgs& a)
-{
-  const float q = product(Running::ref(top), a.c);
-  return Running::large(q) ? (double)Running::ref(top) : (double)q * a.ln2_t;
-}
+// The sum against `top` itself, for the listed tokens, the loss and the statistics, from the one against
+// fl(top c) that the terms of the dense part belong to.
+__device__ __forceinline__ double exact_sum(float top, double all, float c) { return all * exp2(Running::residue(top, c)); }
 __device__ __forceinline__ double factor_of(const DistillArgs& a, int64_t r)
 {
   return (a.row_grad != nullptr ? (double)a.row_grad[r] : 1.0) * a.scale * a.inv_t;
@@ -425,9 +418,9 @@ __global__ __launch_bounds__(64 * W, NV > 8 ? 4 : 8) void distill_rows_kernel(Di
   }
   __syncthreads();  // the dense part is written before the listed tokens'
   if (lead) {
-    const double m = m_of(top, a);
-    write_loss(a, box, r, top, m, all);
-    if (mass != 0) patch(a, box, out, c, mass, m, all, twice);
+    const double s = exact_sum(top, all, a.c);
+    write_loss(a, box, r, top, s);
+    if (mass != 0) patch(a, box, out, c, mass, (double)Running::ref(top), s, twice);
   }
 }
 
@@ -470,9 +463,10 @@ __global__ __launch_bounds__(64 * W, 5) void distill_grad_kernel(DistillArgs a, 
   const int ext_i = piece == 0 ? vs.extra(n) : -1;
   const float ext = ext_i >= 0 ? widen(row + ext_i) : -kInf;
   const float top = a.stats[2 * r];
-  const double m  = m_of(top, a);
+  const double m  = (double)Running::ref(top);
+  const double s  = exp((double)a.stats[2 * r + 1]);
   // against fl(m c), as the terms are
-  const double all = exp((double)a.stats[2 * r + 1] + ((double)Running::ref(top) - m) * a.inv_t);
+  const double all = s * exp2(-Running::residue(top, a.c));
   TeacherBox box(lds, a.k, 0);
   const int lo    = vs.head + from * VEC, hi = vs.head + to * VEC;
   auto mine       = [&](int i) { return (i >= lo && i < hi) || (piece == 0 && i >= 0 && (i < vs.head || i >= vs.head + vs.nv * VEC)); };
@@ -509,7 +503,7 @@ __global__ __launch_bounds__(64 * W, 5) void distill_grad_kernel(DistillArgs a, 
     double p = 0;  // the same token may be listed more than once: every entry writes the whole sum
     for (int o = 0; o < a.k; ++o)
       if (box.index[o] == i) p += box.p[o];
-    Put<T>::st(out + i, (float)(c * (mass * share_of(a, box.z[j], m, all) - p)));
+    Put<T>::st(out + i, (float)(c * (mass * share_of(a, box.z[j], m, s) - p)));
   }
 }
 
@@ -601,8 +595,11 @@ __global__ __launch_bounds__(64 * W, 4) void distill_stream_kernel(DistillArgs a
     __syncthreads();
     joined<W>(max, sum, a.c, top, all);
   }
-  const double m = m_of(top, a);
-  if (lead) write_loss(a, box, r, top, m, all);
+  double s = 0;
+  if (lead) {
+    s = exact_sum(top, all, a.c);
+    write_loss(a, box, r, top, s);
+  }
   if constexpr (GRAD) {
     const double mass = mass_box;
     const double c    = factor_of(a, r);
@@ -630,7 +627,7 @@ __global__ __launch_bounds__(64 * W, 4) void distill_stream_kernel(DistillArgs a
       Put<T>::st(out + ext_i, dense.one(ext));
     }
     __syncthreads();
-    if (lead && !dense.zero) patch(a, box, out, c, mass, m, all, twice);
+    if (lead && !dense.zero) patch(a, box, out, c, mass, (double)Running::ref(top), s, twice);
   }
 }
 
@@ -699,7 +696,6 @@ int run(int dtype, int t_dtype, int64_t n_rows, int64_t n_cols, int64_t ld, int6
   a.t_dtype = t_dtype;
   a.inv_t   = 1.0 / temperature;
   a.scale   = scale;
-  a.ln2_t   = kLn2 * temperature;
   a.c       = (float)(kLog2e / temperature);
   hipStream_t st = static_cast<hipStream_t>(stream);
   switch (dtype) {

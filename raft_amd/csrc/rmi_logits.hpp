@@ -480,8 +480,8 @@ __device__ __forceinline__ float product(float a, float b)
 }
 
 // A running maximum and sum of exp2((x - m) c) of the elements that one thread sees.  The terms are
-// exp2(fma(x, c, -r)) with r = fl(m c): one rounding each, and r's own drops out of the sum's
-// logarithm, which is taken against r.  That rounding is in the exponent, 2^-25 of |r| at most: from
+// exp2(fma(x, c, -r)) with r = fl(m c): one rounding each, and r's own is taken back from the whole
+// sum (residue()).  That rounding is in the exponent, 2^-25 of |r| at most: from
 // |r| = 2^17 on, where it reaches 2^-8 (and 128, beyond which nothing is left of a sum, at 2^32), the
 // difference x - m is taken first.
 struct Running {
@@ -534,12 +534,18 @@ struct Running {
   {
     return (double)(s * moved(m, r, top, product(ref(top), c), c));
   }
+  // The power of two that a sum held against fl(m c) is short of the sum held against m itself, exactly.  With it
+  // c = fl(log2(e) / T) multiplies nothing but distances from m, so that what c is off by does not grow with |m|.
+  __device__ __forceinline__ static double residue(float top, float c)
+  {
+    const float m = ref(top), q = product(m, c);
+    return large(q) ? 0.0 : (double)q - (double)m * (double)c;
+  }
   // log of sum exp(x / T) from all = the sum over the threads of against(top)
   __device__ __forceinline__ static double log_sum(float top, float c, double inv_t, double all)
   {
     if (all == all && fabsf(top) == kInf) return (double)top;
-    const float q = product(ref(top), c);
-    return (large(q) ? (double)ref(top) * inv_t : (double)q * kLn2) + log(all);
+    return (double)ref(top) * inv_t + residue(top, c) * kLn2 + log(all);
   }
 };
 

@@ -64,6 +64,16 @@ def test_distill_far_from_zero(gpu, dtype, far, temperature, calls):
         _distill(_far_rows(far, temperature, n, rng), dtype, temperature, calls, rng)
 
 
+@pytest.mark.parametrize("far,temperature", [(100.0, 1.0), (1e3, 1.0), (1e4, 1.0), (8e4, 1.0), (8e4, 1e-4), (2e4, 50.0)])
+@pytest.mark.parametrize("calls", [1, 2])
+def test_distill_does_not_depend_on_a_common_shift(gpu, far, temperature, calls):
+    """What the constant log2(e) / T is off by counts for the distances from the maximum alone, and a reference's
+    rounding not at all."""
+    rng = np.random.default_rng(3)
+    for n in LENGTHS:
+        _distill(_far_rows(far, temperature, n, rng), "f32", temperature, calls, rng)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("temperature", [1.0, 0.25])
 def test_rows_that_begin_far_below_the_rest(gpu, dtype, temperature):
