@@ -228,14 +228,12 @@ struct Guess {
   __device__ __forceinline__ bool doubtful() const { return !(run.s >= 0.5f && run.s < kMost); }
 };
 
-// dense part of the gradient: f exp((x - m) / T), f = c P / s
-// Results of 16 bits take the factor into the exponent: exp2(x c - r + log2 |f|) is off by some 2^-19, which
-// their own rounding hides, and saves a multiplication per element; fp32 results multiply.
+// dense part of the gradient: f exp((x - m) / T), f = c P / s.  The factor is multiplied, for results of 16
+// bits too: in the exponent (one instruction less an element, no time less) it would be rounded at the size of
+// m c, which 16 bits show from |m| / T = 6000 on.
 template <class T>
 struct Dense {
-  static constexpr bool kFold = sizeof(T) == 2;
   float f, r, ref, c;
-  u32 sign;
   bool large, zero;
   __device__ __forceinline__ Dense(float top, float c_, double factor, double mass, double s) : c(c_)
   {
@@ -245,11 +243,11 @@ struct Dense {
     // a row without a finite logit has q = 0 everywhere; without a teacher its gradient is zero
     zero = mass == 0;
     f    = s == 0 || zero ? 0.0f : (float)(factor * mass) / (float)s;
-    sign = 0;
-    if (kFold && !large) {
-      sign = f < 0 ? 0x80008000u : 0u;
-      r -= __builtin_amdgcn_logf(fabsf(f));  // f = 0: exp2(-inf) = 0
-    }
+  }
+  __device__ __forceinline__ float one(float x) const
+  {
+    if (zero) return 0.0f;
+    return f * __builtin_amdgcn_exp2f(large ? (x - ref) * c : fmaf(x, c, -r));
   }
   __device__ __forceinline__ u32x4 operator()(const u32x4& w) const
   {
@@ -260,26 +258,11 @@ struct Dense {
     if (large) {
 #pragma unroll
       for (int j = 0; j < VEC; ++j) x[j] = f * __builtin_amdgcn_exp2f((x[j] - ref) * c);
-      return pack<T>(x);
-    }
+    } else {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      x[j] = __builtin_amdgcn_exp2f(fmaf(x[j], c, -r));
-      if (!kFold) x[j] *= f;
+      for (int j = 0; j < VEC; ++j) x[j] = f * __builtin_amdgcn_exp2f(fmaf(x[j], c, -r));
     }
-    u32x4 y = pack<T>(x);
-    if constexpr (kFold) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) y[j] ^= sign;
-    }
-    return y;
-  }
-  __device__ __forceinline__ float one(float x) const
-  {
-    if (zero) return 0.0f;
-    if (large) return f * __builtin_amdgcn_exp2f((x - ref) * c);
-    x = __builtin_amdgcn_exp2f(fmaf(x, c, -r));
-    return kFold ? (sign != 0 ? -x : x) : x * f;
+    return pack<T>(x);
   }
 };
 

@@ -106,3 +106,15 @@ def test_many_rows_that_begin_far_below_the_rest(gpu):
     x = rng.normal(0, 1.5, (rows, n))
     x[np.arange(rows), n - 1 - np.arange(rows)] = rng.uniform(20, 95, rows)
     _distill(x, "f32", 1.0, 1, rng, scale=1 / 4096, listed=False)
+
+
+@pytest.mark.parametrize("dtype,far,temperature", [
+    ("f16", 100.0, 1.0), ("f16", 6e3, 1.0), ("f16", 6e4, 1.0), ("f16", 2e4, 1e-3), ("f16", 8e4, 1e-2),
+    ("bf16", 100.0, 1.0), ("bf16", 6e3, 1.0), ("bf16", 5e4, 1.0), ("bf16", 8e4, 1.0), ("bf16", 8e4, 1e-4)])
+@pytest.mark.parametrize("calls", [1, 2])
+def test_16_bit_gradient_of_large_logits(gpu, dtype, far, temperature, calls):
+    """A factor of the gradient that went into the exponent would be rounded at the size of max / T."""
+    rng = np.random.default_rng(4)
+    for n in LENGTHS:
+        for listed in (True, False):
+            _distill(_far_rows(far, temperature, n, rng), dtype, temperature, calls, rng, listed=listed)
