@@ -114,9 +114,11 @@ __device__ __forceinline__ double teacher_norm(const DistillArgs& a, int64_t r, 
   return ref + log(wave_all(sum, AddF{}));
 }
 
-// q of one logit, in 64 bits
+// q of one logit, in 64 bits.  A sum of +inf leaves q = 0 for every finite logit, also where its own exponential
+// passes the largest number.
 __device__ __forceinline__ double share_of(const DistillArgs& a, float z, double m, double s)
 {
+  if (s == (double)kInf) return z == kInf ? (double)__builtin_nanf("") : 0.0;
   return s == 0 ? 0.0 : exp(((double)z - m) * a.inv_t) / s;
 }
 
@@ -243,6 +245,10 @@ struct Dense {
     // a row without a finite logit has q = 0 everywhere; without a teacher its gradient is zero
     zero = mass == 0;
     f    = s == 0 || zero ? 0.0f : (float)(factor * mass) / (float)s;
+    if (s == (double)kInf) {  // exp2(-inf) for every finite logit, however large, and NaN for +inf
+      r     = kInf;
+      large = false;
+    }
   }
   __device__ __forceinline__ float one(float x) const
   {

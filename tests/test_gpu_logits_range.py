@@ -1,6 +1,8 @@
 """The operators over rows of logits where numbers go far: large logits, small temperatures, rows whose
 beginning lies far below the rest, infinities, for every type.  References and tolerances are those of
 tests/_logits.py and tests/test_gpu_logits.py, in which the errors of a softmax are counted."""
+from unittest import mock
+
 import numpy as np
 import pytest
 
@@ -26,6 +28,17 @@ def _far_rows(far, temperature, n, rng):
                      m * rng.random(n) * rng.choice([-1.0, 1.0], n)])
 
 
+_ref_distill = L.ref_distill
+
+
+def _ref_with_infinities(z, t, idx, temperature, *rest):
+    """The reference for rows that hold +inf as well: the sum is +inf, so q = 0 for a finite logit whatever it
+    is.  exp(z / T) itself passes the largest 64-bit number from z / T = 710 on, and inf / inf is NaN."""
+    z = z.astype(np.float64)
+    beside = np.isposinf(z).any(axis=1, keepdims=True) & np.isfinite(z)
+    return _ref_distill(np.where(beside, np.minimum(z, 0.0), z), t, idx, temperature, *rest)
+
+
 def _distill(x, dtype, temperature, calls, rng, k=8, scale=None, listed=True):
     """Loss and gradient against the 64-bit reference; the teacher lists the maximum, or only others."""
     view, _ = G._put(x, dtype, pad=len(x[0]) % 3)
@@ -38,7 +51,8 @@ def _distill(x, dtype, temperature, calls, rng, k=8, scale=None, listed=True):
     else:
         idx = np.where(idx == best[:, None], -1, idx)
     t = temperature * rng.normal(0, 2, (rows, k))
-    G._check_distill(view, t, idx.astype(np.int32), temperature, scale or temperature, calls=calls)
+    with mock.patch.object(L, "ref_distill", _ref_with_infinities):
+        G._check_distill(view, t, idx.astype(np.int32), temperature, scale or temperature, calls=calls)
 
 
 # |max| / T where the product with log2(e) / T leaves no bits for a softmax: its rounding is 2^-8 and more
@@ -118,3 +132,61 @@ def test_16_bit_gradient_of_large_logits(gpu, dtype, far, temperature, calls):
     for n in LENGTHS:
         for listed in (True, False):
             _distill(_far_rows(far, temperature, n, rng), dtype, temperature, calls, rng, listed=listed)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("calls", [1, 2])
+def test_infinite_logit_beside_large_ones(gpu, dtype, calls):
+    """A logit of +inf leaves q = 0 for all others, however large, and NaN for itself."""
+    rng = np.random.default_rng(7)
+    for n in LENGTHS:
+        x = rng.normal(0, 2, (4, n))
+        x[0] += 120.0
+        x[1] -= 400.0
+        x[2, rng.random(n) < 0.5] = 500.0
+        x[3, rng.random(n) < 0.5] = -INF
+        x[np.arange(4), rng.integers(0, n, 4)] = INF
+        for temperature in (1.0, 0.8):
+            _distill(x, dtype, temperature, calls, rng)
+            _distill(x, dtype, temperature, calls, rng, listed=False)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("calls", [1, 2])
+def test_distill_patterns(gpu, dtype, calls):
+    """Infinities, NaN, lowest values, equal ones, in every type of the gradient."""
+    rng = np.random.default_rng(8)
+    for n in LENGTHS:
+        x = G._patterns(n, rng)
+        x[np.abs(x) == 3.3e38] *= {"f32": 1.0, "f16": 65504 / 3.3e38, "bf16": 1.0}[dtype]
+        _distill(x, dtype, 1.0, calls, rng)
+        _distill(x, dtype, 0.5, calls, rng, listed=False)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("calls", [1, 2])
+@pytest.mark.parametrize("n", [40, 5000, 140000])
+def test_16_bit_masked_and_odd_values(gpu, dtype, calls, n):
+    """-inf, the lowest value, NaN and +inf among 16-bit logits; listed tokens among them or not."""
+    rng = np.random.default_rng(n)
+    low = -65504.0 if dtype == "f16" else -3.3e38
+    x = rng.normal(0, 1, (10, n))
+    idx = np.array([rng.permutation(n)[:6] for _ in range(10)], dtype=np.int32)
+    t = rng.normal(0, 2, (10, 6))
+    x[0, rng.random(n) < 0.5] = -INF
+    x[0, idx[0]] = 1.0
+    x[1, idx[1, 0]] = -INF
+    x[2] = -INF
+    x[2, idx[2]] = rng.normal(0, 1, 6)
+    x[3, rng.random(n) < 0.9] = low
+    x[4] = low
+    x[5, n // 2] = NAN
+    x[6, n // 3] = INF
+    x[7] = -INF
+    idx[7] = -1
+    x[8, 0] = NAN
+    idx[8] = -1
+    t[9, 1] = -INF
+    view, _ = G._put(x, dtype)
+    G._check_distill(view, t, idx, 1.0, 1.0, calls=calls, t_dtype=dtype)
+    G._check_distill(view, t, idx, 0.25, 1.0, calls=calls, t_dtype=dtype)
