@@ -403,7 +403,8 @@ RMI_API int rmi_top_k(int dtype,
  * logit r near the row's maximum and log(sum_v exp((z_v - r) / T)), what rmi_distill_grad wants) and `grad`
  * ([n_rows][n_cols] of dtype, rows ld_grad apart), which then costs one pass over the logits instead
  * of two.  rmi_distill_grad writes `grad` from the stats of an earlier rmi_distill_loss with the same
- * logits, teacher and temperature.  `grad` may be the logits' own memory if ld_grad = ld.
+ * logits, teacher and temperature.  `grad` may be the logits' own memory if ld_grad = ld
+ * (RMI_ERR_BAD_SHAPE if it is not); it must not overlap them in any other way.
  * 0 <= k <= RMI_DISTILL_MAX. */
 #define RMI_DISTILL_MAX 1024
 RMI_API int rmi_distill_loss(int dtype,

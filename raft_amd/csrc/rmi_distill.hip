@@ -669,6 +669,8 @@ int run(int dtype, int t_dtype, int64_t n_rows, int64_t n_cols, int64_t ld, int6
   if (rc != RMI_OK) return rc;
   if (k < 0 || k > RMI_DISTILL_MAX) return RMI_ERR_BAD_SHAPE;
   if (a.grad != nullptr && n_rows > 1 && a.ld_grad < n_cols) return RMI_ERR_BAD_SHAPE;
+  // in place every row lies where it was: with another distance one row's gradient would run over another's logits
+  if (a.grad != nullptr && a.grad == a.z && n_rows > 1 && n_cols > 0 && a.ld_grad != ld) return RMI_ERR_BAD_SHAPE;
   if (!(temperature >= kMinTemperature && temperature <= kMaxTemperature) || !(scale - scale == 0))
     return RMI_ERR_UNSUPPORTED;
   if (n_rows == 0 || (n_cols == 0 && a.loss == nullptr)) return RMI_OK;
