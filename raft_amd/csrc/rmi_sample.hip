@@ -90,7 +90,7 @@ struct Settings {
     if (greedy) temperature = 1.0f;
     top_k = greedy ? 1 : (a.top_k != nullptr ? a.top_k[r] : 0);
     top_p = !greedy && a.top_p != nullptr ? a.top_p[r] : 1.0f;
-    if (!(top_p < 1.0f)) top_p = 1.0f;
+    top_p = top_p < 1.0f ? (top_p > 0.0f ? top_p : 0.0f) : 1.0f;  // a negative mass has no whole number
     min_p = !greedy && a.min_p != nullptr ? a.min_p[r] : 0.0f;
     min_p = min_p > 0.0f ? (min_p < 1.0f ? min_p : 1.0f) : 0.0f;
     u     = a.u[r];

@@ -190,3 +190,15 @@ def test_16_bit_masked_and_odd_values(gpu, dtype, calls, n):
     view, _ = G._put(x, dtype)
     G._check_distill(view, t, idx, 1.0, 1.0, calls=calls, t_dtype=dtype)
     G._check_distill(view, t, idx, 0.25, 1.0, calls=calls, t_dtype=dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [9, 5000, 40003])
+def test_sample_keeps_one_token_below_any_mass(gpu, dtype, n):
+    """top_p at and below zero leaves the token that ranks first, with top_k and min_p or without."""
+    rng = np.random.default_rng(n)
+    view, _ = G._put(rng.normal(0, 0.5, (5, n)), dtype)
+    top_p = np.array([0.0, -0.0, -1e-30, -1e30, -INF])
+    for _ in range(2):
+        G._check_sample(view, rng.random(5), top_p=top_p)
+        G._check_sample(view, rng.random(5), top_p=top_p, top_k=np.full(5, 400), min_p=np.full(5, 1e-3))
