@@ -362,7 +362,9 @@ RMI_API int rmi_cov(int dtype,
  * rows start `ld` elements apart (ld >= n_cols; what lies between a row's end and the next row is
  * never read or written).  n_cols is below 2^31 - 65536 and n_rows below 2^31; an element's offset
  * may pass 32 bits.  Rows of other element types are refused with RMI_ERR_UNSUPPORTED, a
- * temperature outside [1e-6, 1e6] likewise.  Results are the same bits every time.
+ * temperature outside [1e-6, 1e6] likewise.  Results are the same bits every time for the same shape; log-sum-exps,
+ * losses and gradients may differ in their last bits between shapes, as the number of rows says how many waves a row
+ * gets.  Values, indices and tokens do not depend on it.
  * None of them has a counterpart in the reference. */
 
 /* The k elements of every row that rank first, in rank order: larger values first, NaN behind
@@ -400,7 +402,7 @@ RMI_API int rmi_top_k(int dtype,
  * +inf (q = 0, NaN at the place itself).  Logits that are all -inf have q = 0.  The same token may be listed more than once.
  *
  * rmi_distill_loss writes `loss`, and what the caller asks for of the rest: `stats`[n_rows][2] (a
- * logit r near the row's maximum and log(sum_v exp((z_v - r) / T)), what rmi_distill_grad wants) and `grad`
+ * logit r near the row's maximum and log(sum_v exp((z_v - r) / T)), in fp32, what rmi_distill_grad wants) and `grad`
  * ([n_rows][n_cols] of dtype, rows ld_grad apart), which then costs one pass over the logits instead
  * of two.  rmi_distill_grad writes `grad` from the stats of an earlier rmi_distill_loss with the same
  * logits, teacher and temperature.  `grad` may be the logits' own memory if ld_grad = ld
@@ -456,8 +458,9 @@ RMI_API int rmi_distill_grad(int dtype,
  * its sum; a u below 0 or NaN counts as 0, one of 1 or more takes the last token left.  `logprob`, if not
  * NULL, gets the log of the token's share of what is left.  A row with nothing to choose from (also
  * n_cols = 0) gets token -1 and logprob -inf.  The weights exp((x - max) / T) are held as whole
- * multiples of 2^-(62 - ceil(log2(n_cols))), at most 2^-50, of the largest one, so that all sums of them are
- * exact; tokens of less weight than half of that are never chosen.  The workspace follows the rules of
+ * multiples of 2^-min(50, 62 - ceil(log2(n_cols))) of the largest one, each right to 2^-42 of itself before it
+ * is rounded; all sums of them are exact, so no result depends on their order.  Tokens of less weight than half such a
+ * multiple are never chosen.  The workspace follows the rules of
  * rmi_reduce: rmi_sample_workspace_bytes bytes, 16-byte aligned, no initialisation needed, its first
  * RMI_WORKSPACE_TICKET_BYTES bytes left alone; calls that share one are ordered on one stream. */
 RMI_API size_t rmi_sample_workspace_bytes(int dtype, int64_t n_rows, int64_t n_cols);

@@ -7,8 +7,9 @@
 //
 // Memory is the bound: with the gradient a row is read once and written once where a workgroup's registers
 // hold it, which is why rows are not split (q needs the whole row's s).  Measured: 4096 x 32000 bf16 100 us (83 at
-// the rate of a copy, 6.5 TB/s); 4096 x 131072 bf16 394 us (332).  In two calls the row is read twice: 1000 x
-// 50001 f32 108 us (90).
+// the rate of a copy, 6.5 TB/s); 4096 x 131072 bf16 393 us (332).  In two calls the row is read twice: 1000 x
+// 50001 f32 109 us (90).  Rows beyond the registers are read twice in one call: 4096 x 152064 bf16 523 us (385),
+// 1024 x 131072 f32 240 us (167).
 #include "rmi_logits.hpp"
 #include "rmi_normalize.hpp"
 
@@ -415,7 +416,7 @@ __global__ __launch_bounds__(64 * W, NV > 8 ? 4 : 8) void distill_rows_kernel(Di
 
 // The gradient from the statistics of an earlier forward pass: nothing joins a row's parts, so every
 // workgroup takes one piece of a row, NV vectors a thread, in the order of memory.  (A workgroup that walks
-// a whole row keeps a thousand rows open at once: 1000 x 50001 f32: 92 us against 77.  Six
+// a whole row keeps a thousand rows open at once: 1000 x 50001 f32: 92 us against 77, and 72 now.  Six
 // waves a SIMD leave it too few registers by five, which costs 4 us.)  Its first wave works the teacher's probabilities
 // out again and corrects the listed tokens that lie in the piece.
 template <class T, int W, int NV>

@@ -1,15 +1,19 @@
 // rmi_sample / rmi_sample_workspace_bytes (include/rmi_reduce.h): one token of every row of
 // logits, drawn with a given random number after temperature, top-k, top-p and min-p.
 //
-//   w_v = round(2^bits exp((x_v - max) / T)),  K = what top_k, top_p, min_p and the mask leave,
+//   w_v = 2^bits exp((x_v - max) / T), right to 2^-42 of itself and rounded to a whole number,
+//   K = what top_k, top_p, min_p and the mask leave,
 //   token = the least v with sum_{v' in K, v' <= v} w_v' > u sum_{K} w
 //
-// The token depends on sums over the row being right to the last unit, so weights are whole numbers and sums of
+// The token must not depend on how a row is summed, so weights are whole numbers: sums of
 // them are exact in any order.  One pass bound by memory decides every row whose kept tokens are few (greedy, top_k,
 // a peaked nucleus).  The others cost an exact pass over all weights, some 20 vector instructions an element in
-// 64 bits: that is bound by the vector units of the one CU that has the row (131072 elements: 20 us), and for a wide
-// nucleus a count of the distances before it.  Measured, 131072 tokens: one row of top_k and top_p 14 us, 256 rows of
+// 64 bits on the one CU that has the row (131072 elements: 20 us, half of the time in vector instructions), and for a wide
+// nucleus a count of the distances before it.  Measured, 131072 tokens: one row of top_k and top_p 15 us, 256 rows of
 // bf16: greedy 17, top_k 24, temperature alone 42, nucleus 89, nucleus with min_p 73 us (11.5 to read).
+// The general way, for what neither decides, takes 400 us and more for such a row: top_k above 64 a wave (1024; 512
+// in batches of more rows than CUs, 256 for rows of up to 1024 vectors), a top_p within some 5e-4 of 1, whose window reaches the row's light end, +inf, and
+// more ties than the candidates have room for.
 #include "rmi_logits.hpp"
 
 namespace rmi {
@@ -47,7 +51,7 @@ struct Undecided {
 // is split or in which order it is added up, and they are exact.  n_cols * 2^bits stays below 2^63.
 //
 // With t = (x - m) log2(e) / T in 64 bits: t = k / 256 + f, 2^t = 2^(k >> 8) * table[k & 255] * 2^f,
-// |f| <= 1/512, and 2^f = 1 + f l + (f l)^2 / 2 + (f l)^3 / 6 with l = ln 2, off by (f l)^4 / 24 < 2^-42 / 24.
+// |f| <= 1/512, and 2^f = 1 + f l + (f l)^2 / 2 + (f l)^3 / 6 with l = ln 2, off by (f l)^4 / 24 < 2^-42.6.
 // The last product adds 2^52, so the rounded weight stands in the low bits of the result.
 constexpr int kTable = 256;
 struct Weights {

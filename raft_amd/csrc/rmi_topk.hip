@@ -4,8 +4,9 @@
 // A row has to be read once; nothing else is large, so memory is the bound (a read of this chip: 7.1 TB/s).
 // Any k elements give a threshold that the k-th cannot lie below, and in a long row few elements pass one that was
 // found early: the pass costs a maximum and a comparison a vector.  The log-sum-exp is summed in the same pass
-// against a reference near the maximum.  Measured: 4096 x 32000 bf16, k 64 with the sum: 58 us (39 to
-// read); 1024 x 131072 f32, k 256: 107 us (78); one row of 32000 bf16: 8 us, all of it launch and steps.
+// against a reference near the maximum.  Measured: 4096 x 32000 bf16, k 64 with the sum: 60 us (39 to
+// read; vector instructions are issued in two thirds of the cycles); 1024 x 131072 f32, k 256: 107 us (78); one row of
+// 32000 bf16: 9 us, all of it launch and steps.
 #include "rmi_logits.hpp"
 #include "rmi_normalize.hpp"
 

@@ -169,7 +169,8 @@ def distill_loss(x: torch.Tensor, t_values: torch.Tensor, t_indices: torch.Tenso
                  row_grad: torch.Tensor | None = None) -> None:
     """Run rmi_distill_loss on the current torch stream: the loss of every row of student logits
     against a teacher's stored best logits; `stats` ([rows, 2]) for distill_grad, or the gradient at
-    once in `grad`, which may be `x`."""
+    once in `grad`, which may be `x`.  Autograd records nothing here: logits that came out of a model
+    take the gradient on by `x.backward(grad)`."""
     d, n_rows, n_cols, ld = _logits(x)
     device = x.get_device()
     _call("rmi_distill_loss", device, d, _dtype_of(t_values, "t_values"), n_rows, n_cols, ld, t_values.shape[-1],
@@ -182,7 +183,8 @@ def distill_grad(x: torch.Tensor, t_values: torch.Tensor, t_indices: torch.Tenso
                  grad: torch.Tensor, *, temperature: float = 1.0, scale: float = 1.0,
                  teacher_lse: torch.Tensor | None = None, row_grad: torch.Tensor | None = None) -> None:
     """Run rmi_distill_grad on the current torch stream: the gradient of an earlier distill_loss from
-    its `stats`, for the gradient `row_grad` of every row's loss (None: ones)."""
+    its `stats`, for the gradient `row_grad` of every row's loss (None: ones); for use in a backward
+    pass of the caller's own, as autograd records nothing of either call."""
     d, n_rows, n_cols, ld = _logits(x)
     device = x.get_device()
     _call("rmi_distill_grad", device, d, _dtype_of(t_values, "t_values"), n_rows, n_cols, ld, t_values.shape[-1],
